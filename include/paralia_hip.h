@@ -225,6 +225,65 @@ long long pl_dgemv_noalloc_max_doubles(void);
 int pl_dgemv_noalloc(char trans, long M, long N, double alpha, const double* A, long lda, const double* x, long incx,
                      double beta, double* y, long incy, void* stream);
 
+/* ---- operators of linear layers and of their training (device pointers, no synchronisation, no allocation) ----
+ * They have no counterpart in the reference.  Matrices are column-major like everywhere in this library: a row-major
+ * activation [tokens][features] is a features x tokens matrix, a row-major weight [out][in] an in x out one, so the
+ * forward product of a linear layer is transA = 'T' (weight), transB = 'N' (input), M = out, N = tokens, K = in.
+ * type: the element type of every operand that is not said to have another.  Products of 16-bit operands are summed in 32
+ * bits; everything behind the product is computed in 32 bits (64 for fp64) and rounded once. */
+enum { PL_TYPE_F64 = 0, PL_TYPE_F32 = 1, PL_TYPE_F16 = 2, PL_TYPE_BF16 = 3 };
+enum { PL_ACT_NONE = 0, PL_ACT_RELU = 1, PL_ACT_GELU = 2 /* z Phi(z) */, PL_ACT_GELU_TANH = 3 /* its tanh form */, PL_ACT_SILU = 4 };
+
+typedef struct pl_epilogue {
+  const void* bias;    /* M elements, added to every column of the product; null: none */
+  int activation;      /* PL_ACT_* */
+  int type_D;          /* type of C and D: the operands', or PL_TYPE_F32 with 16-bit operands */
+  void* preact;        /* M x N: where z, the value in front of the activation, goes for the backward pass; null: nowhere */
+  long ld_preact;
+} pl_epilogue;
+
+/* D <- act(z) + beta*C with z = alpha*op(A)*op(B) + bias.  beta == 0 never reads C; alpha == 0 or K == 0 never reads A
+ * and B.  D may be C itself (same pointer and leading dimension), otherwise no output may overlap another operand.
+ * With beta = 1, no activation and C = D this accumulates a weight gradient (16-bit operands: into fp32, if type_D says
+ * so).  workspace: pl_gemm_epilogue_workspace_bytes(type, transA, transB, M, N, K, 0) bytes, 16-byte aligned (null where
+ * that is 0); it must not be shared by calls that may overlap, and a captured graph keeps using the one it was given. */
+long pl_gemm_epilogue_workspace_bytes(int type, char transA, char transB, long M, long N, long K, int with_dbias);
+int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda, const void* B,
+                     long ldb, const pl_epilogue* epilogue, double beta, const void* C, long ldc, void* D, long ldd, void* workspace,
+                     long workspace_bytes, void* stream);
+
+/* D <- (alpha*op(A)*op(B) + beta*C) .* act'(Z), the gradient that a following layer's product sends back through this
+ * layer's activation, Z being what pl_gemm_epilogue left in preact; dbias(m) <- sum over n of D(m, n) before its
+ * rounding (null: not wanted; M elements).  relu'(0) is 0.  PL_ACT_NONE does not read Z.  D may be C or Z itself.
+ * workspace: as above, with_dbias = 1 where dbias is given. */
+int pl_gemm_epilogue_grad(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda,
+                          const void* B, long ldb, int activation, const void* Z, long ldz, double beta, const void* C, long ldc,
+                          void* D, long ldd, void* dbias, void* workspace, long workspace_bytes, void* stream);
+
+/* dZ <- dY .* act'(Z) and dbias(m) <- sum over n of dZ(m, n) before its rounding, on M x N matrices: the gradient of bias
+ * and activation where dY is an operand.  dZ may be dY or Z itself, or null where only dbias is wanted; dbias may be
+ * null.  N == 0 leaves a dbias of zeros.  workspace (only with dbias): pl_bias_act_grad_workspace_bytes bytes, 16-byte
+ * aligned.  The order of the sums depends only on the shape and the type, here and above. */
+long pl_bias_act_grad_workspace_bytes(int type, long M, long N);
+int pl_bias_act_grad(int type, int activation, long M, long N, const void* dY, long lddy, const void* Z, long ldz, void* dZ, long lddz,
+                     void* dbias, void* workspace, long workspace_bytes, void* stream);
+
+/* *norm <- sqrt of the sum of the squares of all elements of n tensors: tensor i has counts[i] elements of types[i] at
+ * grads[i].  The three lists are host arrays that are free again when the call returns; the tensors, norm (one double) and
+ * the workspace (pl_grad_norm_workspace_bytes(n) bytes, 16-byte aligned) are in device memory.  Squares are formed and
+ * added in 64 bits, in an order that depends only on counts.  Infinities and NaN come through. */
+long pl_grad_norm_workspace_bytes(long n);
+int pl_grad_norm(long n, const void* const* grads, const long long* counts, const int* types, double* norm, void* workspace,
+                 long workspace_bytes, void* stream);
+/* outs[i] <- grads[i] * min(1, max_norm / (*norm + eps)) with a norm that is on the device already (of several GPUs'
+ * gradients, say).  outs[i] may be grads[i] itself; any other overlap of an output with a tensor of the list is refused,
+ * the same tensor listed twice among them.  max_norm and eps must not be negative.  A NaN norm makes every element NaN. */
+int pl_grad_clip(long n, const void* const* grads, const long long* counts, const int* types, void* const* outs, double max_norm,
+                 double eps, const double* norm, void* stream);
+/* both in one call, one launch fewer */
+int pl_grad_norm_clip(long n, const void* const* grads, const long long* counts, const int* types, void* const* outs, double max_norm,
+                      double eps, double* norm, void* workspace, long workspace_bytes, void* stream);
+
 /* ---- routines: plain-C faces of Library_scheduler/include/PARALiA.hpp:33-72 ----
  * Operands may be host (pinned or pageable) or device pointers; the library detects which.  Calls return
  * after the result has reached the caller's buffer.  T > 0 / cache_limit > 0 preset the tile size and the

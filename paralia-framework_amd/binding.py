@@ -6,6 +6,8 @@ import subprocess
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libparalia.so")
 PL_PLAN_MAX_WAITS = 12
+PL_TYPE_F64, PL_TYPE_F32, PL_TYPE_F16, PL_TYPE_BF16 = range(4)
+PL_ACT_NONE, PL_ACT_RELU, PL_ACT_GELU, PL_ACT_GELU_TANH, PL_ACT_SILU = range(5)
 PL_PLAN_ROW = 14 + PL_PLAN_MAX_WAITS
 
 
@@ -28,6 +30,14 @@ class gemm_fit(C.Structure):
                 ("f32_large_fixed_us", (C.c_double * 2) * 4), ("edge_rounds", C.c_double * 2)]
 
 
+class epilogue(C.Structure):
+    """pl_epilogue of include/paralia_hip.h."""
+    _fields_ = [("bias", C.c_void_p), ("activation", C.c_int), ("type_d", C.c_int), ("preact", C.c_void_p), ("ld_preact", C.c_long)]
+
+    def __init__(self, bias=None, activation=0, type_d=PL_TYPE_F64, preact=None, ld_preact=0):
+        super().__init__(bias, activation, type_d, preact, ld_preact)
+
+
 def build_library(jobs=8):
     """Compile every HIP and C++ source for gfx950 (hipcc cross-compiles without a GPU)."""
     subprocess.run(["make", "-C", PKG_DIR, "-j%d" % jobs], check=True)
@@ -37,6 +47,7 @@ _lib = None
 
 _vp, _l, _ll, _i, _d, _f, _c = C.c_void_p, C.c_long, C.c_longlong, C.c_int, C.c_double, C.c_float, C.c_char
 _pi = C.POINTER(C.c_int)
+_pp, _pll = C.POINTER(C.c_void_p), C.POINTER(C.c_longlong)
 
 _SIGS = {
     "pl_last_error": (C.c_char_p, []),
@@ -96,6 +107,15 @@ _SIGS = {
     "pl_dgemv": (_i, [_c, _l, _l, _d, _vp, _l, _vp, _l, _d, _vp, _l, _vp, _vp]),
     "pl_dgemv_noalloc_max_doubles": (_ll, []),
     "pl_dgemv_noalloc": (_i, [_c, _l, _l, _d, _vp, _l, _vp, _l, _d, _vp, _l, _vp]),
+    "pl_gemm_epilogue_workspace_bytes": (_l, [_i, _c, _c, _l, _l, _l, _i]),
+    "pl_gemm_epilogue": (_i, [_i, _c, _c, _l, _l, _l, _d, _vp, _l, _vp, _l, C.POINTER(epilogue), _d, _vp, _l, _vp, _l, _vp, _l, _vp]),
+    "pl_gemm_epilogue_grad": (_i, [_i, _c, _c, _l, _l, _l, _d, _vp, _l, _vp, _l, _i, _vp, _l, _d, _vp, _l, _vp, _l, _vp, _vp, _l, _vp]),
+    "pl_bias_act_grad_workspace_bytes": (_l, [_i, _l, _l]),
+    "pl_bias_act_grad": (_i, [_i, _i, _l, _l, _vp, _l, _vp, _l, _vp, _l, _vp, _vp, _l, _vp]),
+    "pl_grad_norm_workspace_bytes": (_l, [_l]),
+    "pl_grad_norm": (_i, [_l, _pp, _pll, _pi, _vp, _vp, _l, _vp]),
+    "pl_grad_clip": (_i, [_l, _pp, _pll, _pi, _pp, _d, _d, _vp, _vp]),
+    "pl_grad_norm_clip": (_i, [_l, _pp, _pll, _pi, _pp, _d, _d, _vp, _vp, _l, _vp]),
     "PARALiA_last_error": (C.c_char_p, []),
     "PARALiA_dgemm": (_i, [_c, _c, _l, _l, _l, _d, _vp, _l, _vp, _l, _d, _vp, _l, _l, _ll, C.POINTER(atc_info)]),
     "PARALiA_sgemm": (_i, [_c, _c, _l, _l, _l, _f, _vp, _l, _vp, _l, _f, _vp, _l, _l, _ll, C.POINTER(atc_info)]),
