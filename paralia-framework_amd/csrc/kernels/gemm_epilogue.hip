@@ -39,6 +39,9 @@ __device__ __forceinline__ floatx16 mfma16(short8_t a, short8_t b, floatx16 c, f
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// s_waitcnt: at most n vector memory operations left, nothing else waited for
+constexpr int vm_wait(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+
 // A panel of EXT rows of op(A) (columns of op(B)) by H_BK values of k, in 16-byte granules of 8 elements; 64 granules, what
 // one request of a wave loads, are a piece.
 template <bool KMAJOR, int EXT> struct HalfPanel {
@@ -75,6 +78,24 @@ __device__ __forceinline__ void request_offsets(unsigned (&off)[P::NV], long ld,
     else g = min(g, (rows_left - 1) >> 3);
     off[i] = (unsigned)row * (unsigned)ld * 2u + (unsigned)g * 16u;
   }
+}
+
+// The same for loads through registers, which need no alignment.  MN-major: from the start of the panel's first k-row, of
+// which `first` is the tile's first element and `extent` the number of elements (at least 8); the granule that reaches
+// past them is read 8 elements short of their end, and its first elements, as many as this returns, are dropped later.
+template <typename P, bool KMAJOR>
+__device__ __forceinline__ int load_offsets(unsigned (&off)[P::NV], long ld, int first, int extent, int tid) {
+  int row, g;
+  P::holds(tid / 64, tid % 64, row, g);   // (the same granule for all of a thread's vectors)
+  const int start = KMAJOR ? g * 8 : min(first + g * 8, extent - 8);
+#pragma unroll
+  for (int i = 0; i < P::NV; ++i) {
+    int r, unused;
+    P::holds(tid / 64 + 4 * i, tid % 64, r, unused);
+    if (KMAJOR) r = min(r, extent - first - 1);
+    off[i] = (unsigned)r * (unsigned)ld * 2u + (unsigned)start * 2u;
+  }
+  return KMAJOR ? 0 : min(8, first + g * 8 - start);
 }
 
 // A wave-uniform pointer in scalar registers, so that a request is "scalar base + 32-bit lane offset".
@@ -124,24 +145,9 @@ __device__ __forceinline__ void fetch_panel(const short* __restrict__ base, long
   for (int i = 0; i < P::NV; ++i) {
     int row, g;
     P::holds(tid / 64 + 4 * i, tid % 64, row, g);
-    const int start = min(g * 8, contig - 8);
-    regs[i] = *reinterpret_cast<const Loose<short>::type*>(base + (long)min(row, strided - 1) * ld + start);
-  }
-  if (contig < P::PER_ROW * 8) {
-#pragma unroll
-    for (int i = 0; i < P::NV; ++i) {
-      int row, g;
-      P::holds(tid / 64 + 4 * i, tid % 64, row, g);
-      regs[i] = drop_front(regs[i], min(8, max(0, g * 8 - (contig - 8))));
-    }
-  }
-  if (!KMAJOR && strided < H_BK) {
-#pragma unroll
-    for (int i = 0; i < P::NV; ++i) {
-      int row, g;
-      P::holds(tid / 64 + 4 * i, tid % 64, row, g);
-      regs[i] &= (short)((row - strided) >> 31);
-    }
+    regs[i] = *reinterpret_cast<const Loose<short>::type*>(base + (long)min(row, strided - 1) * ld + min(g * 8, contig - 8));
+    regs[i] = drop_front(regs[i], min(8, max(0, g * 8 - (contig - 8))));
+    if (!KMAJOR) regs[i] &= (short)((row - strided) >> 31);
   }
 }
 template <typename P>
@@ -195,9 +201,9 @@ template <bool KMAJOR, int EXT> struct Reader {
   }
 };
 
-// fast: both operands 16-byte aligned with leading dimensions that the request offsets span.  kchunk: split K (0: no).
-template <typename T, typename TD, bool AK, bool BKM, int BM, int BN, bool GRAD>
-__global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void half_product_kernel(int M, int N, int K, const short* __restrict__ A, long lda,
+// fast: 2: both operands can be requested, 1: leading dimensions within the offsets' range, 0: neither.  kchunk: split K (0: no).
+template <typename T, typename TD, bool AK, bool BKM, int BM, int BN, int STAGES, bool GRAD>
+__global__ __launch_bounds__(H_THREADS, (BM * BN * STAGES <= 128 * 128 * 2 ? 2 : 1)) void half_product_kernel(int M, int N, int K, const short* __restrict__ A, long lda,
                                                                                                const short* __restrict__ B, long ldb, int gm, int gn, int fast,
                                                                                                int kchunk, Epilogue ep) {
   using PA = HalfPanel<AK, BM>;
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void hal
   constexpr int STAGE = PA::ELEMS + PB::ELEMS;
   constexpr int EP_LD = WM + 4;                       // floats per column of the epilogue's staging area
   static_assert(4 * 32 * EP_LD * 4 <= 2 * STAGE * 2, "the epilogue stages in the panels' memory");
-  __shared__ __attribute__((aligned(1024))) short smem[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) short smem[STAGES * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (wave & 1) * WM, wn = (wave >> 1) * WN;
@@ -237,18 +243,25 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void hal
 
   const Reader<AK, BM> ra(wm, lane);
   const Reader<BKM, BN> rb(wn, lane);
-  auto multiply = [&](const short* xs) {
+  auto multiply = [&](const short* xs) {   // the operands of a step are read in front of the MFMAs of the one before it
+    constexpr int SETS = BM > 128 ? 1 : 2;   // (the large tile comes here for the rest of K only, and has no registers to spare)
+    short8_t a[SETS][NBM], b[SETS][NBN];
+    auto read = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < NBM; ++i) a[s % SETS][i] = ra.read(xs, i, s);
+#pragma unroll
+      for (int j = 0; j < NBN; ++j) b[s % SETS][j] = rb.read(xs + PA::ELEMS, j, s);
+    };
+    if (SETS > 1) read(0);
 #pragma unroll
     for (int s = 0; s < H_BK / 16; ++s) {
-      short8_t a[NBM], b[NBN];
-#pragma unroll
-      for (int i = 0; i < NBM; ++i) a[i] = ra.read(xs, i, s);
-#pragma unroll
-      for (int j = 0; j < NBN; ++j) b[j] = rb.read(xs + PA::ELEMS, j, s);
+      if (SETS == 1) read(s);
+      else if (s + 1 < H_BK / 16) read(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < NBM; ++i)
 #pragma unroll
-        for (int j = 0; j < NBN; ++j) acc[i][j] = mfma16(a[i], b[j], acc[i][j], T());
+        for (int j = 0; j < NBN; ++j) acc[i][j] = mfma16(a[s % SETS][i], b[s % SETS][j], acc[i][j], T());
     }
   };
 
@@ -256,7 +269,7 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void hal
   // it where the extent is not a multiple of 8; behind every k-row but the last that is still the operand's own memory
   // (its leading dimension is a multiple of 8), so the last k-row is left to the guarded step.
   const bool last_row_guarded = (!AK && mrem < BM && (M & 7)) || (!BKM && nrem < BN && (N & 7));
-  const int nfull = fast ? (K - (last_row_guarded ? 1 : 0)) / H_BK : 0;
+  const int nfull = fast == 2 ? (K - (last_row_guarded ? 1 : 0)) / H_BK : 0;
   if (nfull > 0) {
     unsigned oa[PA::NV], ob[PB::NV];
     request_offsets<PA, AK>(oa, lda, mrem, wave, lane);
@@ -275,19 +288,24 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void hal
     constexpr int STEPS = H_BK / 16, READS = NBM + NBN, MFMAS = NBM * NBN, SPREAD = MFMAS > 4 ? MFMAS * 3 / 4 : MFMAS / 2;   // (the reads go out early enough to be done when the step ends)
     // One panel.  The operands of a step are read during the step before it, so the panel's barrier sits in front of its
     // last step: from there on every wave has read all of panel kt, panel kt + 1 is complete, and the requests of panel
-    // kt + 2 may fill panel kt's buffer.  The source is in issue order, an MFMA and then what goes out behind it.
+    // kt + STAGES may fill panel kt's buffer, the first half of them at once, the rest during the next panel's first step.
+    // The source is in issue order, an MFMA and then what goes out behind it.  STEADY: all those panels exist.
     // (__restrict__: a transposing read that the compiler cannot tell from the requests' buffer waits for all of them.)
-    auto panel = [&](int kt, short* __restrict__ cur, short* __restrict__ nxt, bool ask1, bool ask2) __attribute__((always_inline)) {
-      const char* const a1 = uniform_base(Ab + (kt + 1) * a_step);
-      const char* const b1 = uniform_base(Bb + (kt + 1) * b_step);
-      const char* const a2 = uniform_base(Ab + (kt + 2) * a_step);
-      const char* const b2 = uniform_base(Bb + (kt + 2) * b_step);
+    const short* next_a = Ab + (STAGES - 1) * a_step;   // the panel that is being asked for
+    const short* next_b = Bb + (STAGES - 1) * b_step;
+    constexpr int NEWER = (STAGES - 2) * NR;   // requests that may be out when panel kt + 1 has landed
+    auto panel = [&]<bool STEADY>(int kt, short* __restrict__ cur, short* __restrict__ nxt, short* __restrict__ prv) __attribute__((always_inline)) {
+      const bool ask1 = STEADY || kt + STAGES - 1 < nfull, ask2 = STEADY || kt + STAGES < nfull, next = STEADY || kt + 1 < nfull;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         const bool last = s == STEPS - 1;
-        if (last && ask1) {
+        if (last) next_a += a_step, next_b += b_step;
+        const char* const pa = uniform_base(next_a);
+        const char* const pb = uniform_base(next_b);
+        if (last && next) {
           // this wave's part of panel kt + 1 is in LDS (vmcnt), and its last reads of panel kt are done (lgkmcnt)
-          __builtin_amdgcn_s_waitcnt(0x0070);
+          if (ask1) __builtin_amdgcn_s_waitcnt(vm_wait(NEWER) & ~0x0F00);
+          else __builtin_amdgcn_s_waitcnt(vm_wait(0) & ~0x0F00);
           __builtin_amdgcn_s_barrier();
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -295,7 +313,7 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void hal
         for (int m = 0; m < MFMAS; ++m) {
           const int i = m / NBN, j = m % NBN;
           acc[i][j] = mfma16(fa[s & 1][i], fb[s & 1][j], acc[i][j], T());
-          if (!last || ask1) {
+          if (!last || next) {
 #pragma unroll
             for (int e = 0; e < READS; ++e)
               if (e * SPREAD / READS == m) read(last ? nxt : cur, last ? 0 : s + 1, (s + 1) & 1, e);
@@ -303,71 +321,104 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN <= 128 * 128 ? 2 : 1)) void hal
           if (s == 0 && ask1) {
 #pragma unroll
             for (int r = EARLY; r < NR; ++r)
-              if ((r - EARLY) * MFMAS / (NR - EARLY) == m) ask(a1, b1, nxt, r);
+              if ((r - EARLY) * MFMAS / (NR - EARLY) == m) ask(pa, pb, prv, r);
           }
           if (last && ask2) {
 #pragma unroll
             for (int r = 0; r < EARLY; ++r)
-              if (r * MFMAS / EARLY == m) ask(a2, b2, cur, r);
+              if (r * MFMAS / EARLY == m) ask(pa, pb, cur, r);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     };
-    {
-      const char* const a0 = uniform_base(Ab);
-      const char* const b0 = uniform_base(Bb);
 #pragma unroll
-      for (int r = 0; r < NR; ++r) ask(a0, b0, smem, r);
-      const char* const a1 = uniform_base(Ab + a_step);
-      const char* const b1 = uniform_base(Bb + b_step);
-      if (nfull > 1) {
+    for (int q = 0; q < STAGES; ++q) {
+      const char* const a0 = uniform_base(Ab + q * a_step);
+      const char* const b0 = uniform_base(Bb + q * b_step);
+      if (q < nfull) {
 #pragma unroll
-        for (int r = 0; r < EARLY; ++r) ask(a1, b1, smem + STAGE, r);
-        __builtin_amdgcn_s_waitcnt(0x0F70 | EARLY);  // panel 0 has landed, the early requests of panel 1 may be out
-      } else {
-        __builtin_amdgcn_s_waitcnt(0x0F70);
+        for (int r = 0; r < (q == STAGES - 1 ? EARLY : NR); ++r) ask(a0, b0, smem + q * STAGE, r);
       }
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
     }
-    static_assert(EARLY < 16, "the wait counter's low bits");
+    if (nfull >= STAGES) __builtin_amdgcn_s_waitcnt(vm_wait(NEWER + EARLY));   // panel 0 has landed
+    else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    static_assert(NEWER + EARLY < 64, "the wait counter's range");
 #pragma unroll
     for (int e = 0; e < READS; ++e) read(smem, 0, 0, e);
-    short* const even = smem;
-    short* const odd = smem + STAGE;
     int kt = 0;
-    for (; kt + 3 < nfull; kt += 2) {
-      panel(kt, even, odd, true, true);
-      panel(kt + 1, odd, even, true, true);
+    for (; kt + 2 * STAGES - 1 < nfull; kt += STAGES) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u)
+        panel.template operator()<true>(kt + u, smem + u * STAGE, smem + (u + 1) % STAGES * STAGE, smem + (u + STAGES - 1) % STAGES * STAGE);
     }
-    for (; kt < nfull; ++kt)   // the last one to three
-      panel(kt, (kt & 1) ? odd : even, (kt & 1) ? even : odd, kt + 1 < nfull, kt + 2 < nfull);
+    for (; kt < nfull; kt += STAGES) {
+#pragma unroll
+      for (int u = 0; u < STAGES; ++u)
+        if (kt + u < nfull) panel.template operator()<false>(kt + u, smem + u * STAGE, smem + (u + 1) % STAGES * STAGE, smem + (u + STAGES - 1) % STAGES * STAGE);
+    }
     __syncthreads();
   }
-  // The rest of K, and all of it where the operands cannot be requested: through registers, two panels ahead.
-  if (nfull * H_BK < K) {
-    short8_t fa[2][PA::NV], fb[2][PB::NV];
-    const int nk = (K + H_BK - 1) / H_BK;
-    auto fetch = [&](int kt, short8_t (&va)[PA::NV], short8_t (&vb)[PB::NV]) {
-      const int krem = K - kt * H_BK;
-      fetch_panel<PA, AK>(Ab + kt * a_step, lda, AK ? mrem : krem, AK ? krem : M - m0, va, tid);
-      fetch_panel<PB, BKM>(Bb + kt * b_step, ldb, BKM ? nrem : krem, BKM ? krem : N - n0, vb, tid);
-    };
-    // panels nfull - 2 and nfull - 1 are not there: their steps only fetch
-    auto step = [&](int kt, short* xs, short8_t (&va)[PA::NV], short8_t (&vb)[PB::NV]) {
-      if (kt >= nfull) {
-        put<PA>(xs, va, tid);
-        put<PB>(xs + PA::ELEMS, vb, tid);
+  int done = nfull;
+  if constexpr (BM == 128 && STAGES == 2) {   // (the launcher gives such operands to this tile)
+    // Unaligned operands: whole panels through registers, loaded two panels ahead.  No branch between the loads and their
+    // use, which would make every use wait for all loads.
+    if (fast == 1 && K >= H_BK) {
+      unsigned oa[PA::NV], ob[PB::NV];
+      const int drop_a = load_offsets<PA, AK>(oa, lda, m0, M, tid), drop_b = load_offsets<PB, BKM>(ob, ldb, n0, N, tid);
+      const short* const base_a = AK ? Ab : A;
+      const short* const base_b = BKM ? Bb : B;
+      const bool edge_a = !AK && mrem < BM, edge_b = !BKM && nrem < BN;
+      done = K / H_BK;
+      short8_t va[2][PA::NV], vb[2][PB::NV];
+      auto load = [&](int kt, int set) {
+        kt = min(kt, done - 1);
+        const char* const ba = uniform_base(base_a + kt * a_step);
+        const char* const bb = uniform_base(base_b + kt * b_step);
+#pragma unroll
+        for (int i = 0; i < PA::NV; ++i) va[set][i] = *reinterpret_cast<const Loose<short>::type*>(reinterpret_cast<const short*>(ba + oa[i]));
+#pragma unroll
+        for (int i = 0; i < PB::NV; ++i) vb[set][i] = *reinterpret_cast<const Loose<short>::type*>(reinterpret_cast<const short*>(bb + ob[i]));
+      };
+      auto step = [&](int kt, int set) {
+        if (edge_a) {
+#pragma unroll
+          for (int i = 0; i < PA::NV; ++i) va[set][i] = drop_front(va[set][i], drop_a);
+        }
+        if (edge_b) {
+#pragma unroll
+          for (int i = 0; i < PB::NV; ++i) vb[set][i] = drop_front(vb[set][i], drop_b);
+        }
+        short* const xs = smem + set * STAGE;
+        put<PA>(xs, va[set], tid);
+        put<PB>(xs + PA::ELEMS, vb[set], tid);
         __syncthreads();
+        load(kt + 2, set);
+        multiply(xs);
+      };
+      load(0, 0);
+      load(1, 1);
+      for (int kt = 0;; kt += 2) {
+        step(kt, 0);
+        if (kt + 1 >= done) break;
+        step(kt + 1, 1);
+        if (kt + 2 >= done) break;
       }
-      if (kt + 2 < nk) fetch(kt + 2, va, vb);
-      if (kt >= nfull) multiply(xs);
-    };
-    for (int kt = nfull - 2; kt < nk; kt += 2) {
-      step(kt, smem, fa[0], fb[0]);
-      if (kt + 1 < nk) step(kt + 1, smem + STAGE, fa[1], fb[1]);
+      __syncthreads();
     }
+  }
+  // The rest of K, and all of it where leading dimensions leave the offsets' range.
+  for (int kt = done; kt * H_BK < K; ++kt) {
+    short8_t va[PA::NV], vb[PB::NV];
+    const int krem = K - kt * H_BK;
+    fetch_panel<PA, AK>(Ab + kt * a_step, lda, AK ? mrem : krem, AK ? krem : M - m0, va, tid);
+    fetch_panel<PB, BKM>(Bb + kt * b_step, ldb, BKM ? nrem : krem, BKM ? krem : N - n0, vb, tid);
+    put<PA>(smem, va, tid);
+    put<PB>(smem + PA::ELEMS, vb, tid);
+    __syncthreads();
+    multiply(smem);
     __syncthreads();
   }
 
@@ -440,7 +491,6 @@ __device__ __forceinline__ floatx4 mfma16_small(short8_t a, short8_t b, floatx4 
 __device__ __forceinline__ floatx4 mfma16_small(short8_t a, short8_t b, floatx4 c, f16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-constexpr int vm_wait(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }   // at most n vector memory operations left
 
 template <typename T, typename TD, int RB, int NB>
 __global__ __launch_bounds__(FEW_WAVES * 64, 2) void half_few_columns_kernel(int M, int N, int K, const short* __restrict__ A, long lda, const short* __restrict__ B,
@@ -587,29 +637,35 @@ inline HalfPlan plan_half(bool at, bool bt, long M, long N, long K) {
   return best;
 }
 
-// rows of partial bias gradients the 16-bit product leaves
+// rows of partial bias gradients the 16-bit product leaves: two per tile column, or those of the pass
 inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
   return p.splits > 1 || p.tile == 0 ? epilogue_pass_rows(type, M, N) : 2 * ((N + p.tile - 1) / p.tile);
+}
+
+// requests: 16-byte granules, and offsets from a panel's first element in 32 bits (256 rows of a K-major operand, 64 k-rows
+// of an MN-major one)
+inline bool in_offset_range(long lda, long ldb) { return lda < (1L << 22) && ldb < (1L << 22); }
+inline bool can_request(const void* A, long lda, const void* B, long ldb) {
+  return aligned_to(A, 16) && aligned_to(B, 16) && lda % 8 == 0 && ldb % 8 == 0 && in_offset_range(lda, ldb);
 }
 
 template <typename T, typename TD, bool GRAD>
 int launch_half(const HalfPlan& plan, bool at, bool bt, long M, long N, long K, const void* A, long lda, const void* B, long ldb, const Epilogue& ep, hipStream_t stream) {
   const int gm = (int)((M + plan.tile - 1) / plan.tile), gn = (int)((N + plan.tile - 1) / plan.tile);
-  // requests: 16-byte granules, and offsets from a panel's first element in 32 bits (256 rows of a K-major operand, 64
-  // k-rows of an MN-major one)
-  const int fast = aligned_to(A, 16) && aligned_to(B, 16) && lda % 8 == 0 && ldb % 8 == 0 && lda < (1L << 22) && ldb < (1L << 22);
-#define HALF(AKF, BKF, TILE)                                                                                                                       \
-  hipLaunchKernelGGL((half_product_kernel<T, TD, AKF, BKF, TILE, TILE, GRAD>), dim3(gm * gn, plan.splits), dim3(H_THREADS), 0, stream, (int)M, (int)N, \
+  const int fast = can_request(A, lda, B, ldb) ? 2 : in_offset_range(lda, ldb) ? 1 : 0;
+#define HALF(AKF, BKF, TILE, STAGES)                                                                                                                     \
+  hipLaunchKernelGGL((half_product_kernel<T, TD, AKF, BKF, TILE, TILE, STAGES, GRAD>), dim3(gm * gn, plan.splits), dim3(H_THREADS), 0, stream, (int)M, (int)N, \
                      (int)K, (const short*)A, lda, (const short*)B, ldb, gm, gn, fast, plan.kchunk, ep)
-#define HALF_TILE(TILE)                    \
-  do {                                     \
-    if (at && !bt) HALF(true, true, TILE); \
-    else if (at) HALF(true, false, TILE);  \
-    else if (!bt) HALF(false, true, TILE); \
-    else HALF(false, false, TILE);         \
+#define HALF_TILE(TILE, STAGES)                    \
+  do {                                             \
+    if (at && !bt) HALF(true, true, TILE, STAGES); \
+    else if (at) HALF(true, false, TILE, STAGES);  \
+    else if (!bt) HALF(false, true, TILE, STAGES); \
+    else HALF(false, false, TILE, STAGES);         \
   } while (0)
-  if (plan.tile == 256) HALF_TILE(256);
-  else HALF_TILE(128);
+  if (plan.tile == 256) HALF_TILE(256, 2);
+  else if (fast == 2 && (long)gm * gn * plan.splits <= 256) HALF_TILE(128, 4);
+  else HALF_TILE(128, 2);
 #undef HALF_TILE
 #undef HALF
   return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
@@ -625,7 +681,7 @@ inline Workspace workspace_for(int type, bool at, bool bt, long M, long N, long 
   if (type_size(type) == 2) {
     const HalfPlan p = plan_half(at, bt, M, N, K);
     if (p.splits > 1 || p.tile == 0) w.product = round16((long)p.splits * M * N * 4);
-    if (dbias) w.partial = round16(half_partial_rows(p, type, M, N) * M * wide);
+    if (dbias) w.partial = round16(half_partial_rows({p.tile == 256 ? 128 : p.tile, p.splits, 0}, type, M, N) * M * wide);   // (unaligned operands: the small tile)
   } else {
     w.product_ws = round16(pl_gemm_tile_alone_workspace_bytes(at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, type_size(type)));
     w.product = round16(M * N * wide);
@@ -651,8 +707,7 @@ struct Call {
 
 template <typename T> int half_product(const Call& c, const HalfPlan& plan, bool at, bool bt, void* slices, const Epilogue& ep) {
   // few columns: the requests' alignment, whole panels
-  if (at && !bt && !c.grad && c.N <= FEW_MAX_N && c.K > 0 && c.K % H_BK == 0 && aligned_to(c.A, 16) && aligned_to(c.B, 16) && c.lda % 8 == 0 && c.ldb % 8 == 0 &&
-      c.lda < (1L << 25) && c.ldb < (1L << 25)) {
+  if (at && !bt && !c.grad && c.N <= FEW_MAX_N && c.K > 0 && c.K % H_BK == 0 && can_request(c.A, c.lda, c.B, c.ldb)) {
     if (c.type_d == PL_TYPE_F32) return launch_few_columns<T, float>(c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
     return launch_few_columns<T, T>(c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
   }
@@ -719,6 +774,7 @@ int run_product(Call& c) {
   if (es == 2) {
     HalfPlan plan = plan_half(at, bt, M, N, K);
     if (empty) plan.splits = 1, plan.kchunk = 0;
+    if (plan.tile == 256 && !can_request(c.A, c.lda, c.B, c.ldb)) plan.tile = 128;
     rows = half_partial_rows(plan, c.type, M, N);
     rc_ = c.type == PL_TYPE_F16 ? half_product<f16_t>(c, plan, at, bt, ws, ep) : half_product<bf16_t>(c, plan, at, bt, ws, ep);
   } else {
