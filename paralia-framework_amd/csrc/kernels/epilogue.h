@@ -188,39 +188,68 @@ struct Epilogue {
   int act;
 };
 
-// VEC elements of one column of the product, m .. m + VEC - 1 (valid of them inside the matrix), through the epilogue.
-// sums collects the gradient's column values.
+// What an epilogue reads for VEC elements of a column: C, and Z of the gradient.  Loaded in one step and used in another, so
+// that loads can be ahead of their use; the elements beyond `valid` are zero.
+template <typename T, typename TD, bool GRAD, int VEC> struct EpilogueInputs {
+  typedef T zvec __attribute__((ext_vector_type(VEC)));
+  typedef TD cvec __attribute__((ext_vector_type(VEC)));
+  typedef zvec zload __attribute__((aligned(sizeof(T))));
+  typedef cvec cload __attribute__((aligned(sizeof(TD))));
+  cvec c;
+  zvec z;
+  template <typename V, typename L, typename E> static __device__ __forceinline__ V get(const E* p, int valid) {
+    if (valid >= VEC) return *reinterpret_cast<const L*>(p);
+    V v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = e < valid ? p[e] : E(0);
+    return v;
+  }
+  __device__ __forceinline__ void load(const Epilogue& ep, const TD* pc, const T* pz, int valid) {
+    if (valid <= 0) return;
+    if (ep.beta != 0.0) c = get<cvec, cload>(pc, valid);
+    if (GRAD && ep.act != PL_ACT_NONE) z = get<zvec, zload>(pz, valid);
+  }
+};
+
+// VEC elements of one column of the product, `valid` of them inside the matrix, through the epilogue and to D and z at pd
+// and pp.  sums collects the gradient's column values.
 template <typename T, typename TD, bool GRAD, int VEC>
-__device__ __forceinline__ void apply_epilogue(const Epilogue& ep, wide_t<T> (&v)[VEC], const wide_t<T> (&bias)[VEC], long m, long n, int valid,
-                                               wide_t<T> (&sums)[VEC]) {
+__device__ __forceinline__ void apply_epilogue(const Epilogue& ep, const EpilogueInputs<T, TD, GRAD, VEC>& in, wide_t<T> (&v)[VEC], const wide_t<T> (&bias)[VEC], TD* pd,
+                                               T* pp, int valid, wide_t<T> (&sums)[VEC]) {
   using W = wide_t<T>;
   constexpr bool FAST = sizeof(T) == 2;
   const W alpha = (W)ep.alpha, beta = (W)ep.beta;
-  W c[VEC];
-  if (beta != W(0)) load_row<TD, VEC, W>((const TD*)ep.C + n * ep.ldc + m, c, valid);
+  int act = ep.act;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+s"(act));   // compared anew each time: the outcomes, kept over a loop, would not fit the scalar registers
+#endif
   if constexpr (GRAD) {
-    W z[VEC];
-    if (ep.act != PL_ACT_NONE) load_row<T, VEC, W>((const T*)ep.Z + n * ep.ldz + m, z, valid);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      v[e] = alpha * v[e];
-      if (beta != W(0)) v[e] = fma(beta, c[e], v[e]);
+    for (int e = 0; e < VEC; ++e) v[e] = alpha * v[e];
+    if (beta != W(0)) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = fma(beta, (W)in.c[e], v[e]);
     }
-    if (ep.act != PL_ACT_NONE) times_slope<W, FAST, VEC>(v, z, ep.act);
+    if (act != PL_ACT_NONE) {
+      W z[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) z[e] = (W)in.z[e];
+      times_slope<W, FAST, VEC>(v, z, act);
+    }
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
       if (e < valid) sums[e] += v[e];
   } else {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = fma(alpha, v[e], bias[e]);
-    if (ep.preact) store_row<T, VEC, W>((T*)ep.preact + n * ep.ldp + m, v, valid);
-    activate<W, FAST, VEC>(v, ep.act);
+    if (ep.preact) store_row<T, VEC, W>(pp, v, valid);
+    activate<W, FAST, VEC>(v, act);
     if (beta != W(0)) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = fma(beta, c[e], v[e]);
+      for (int e = 0; e < VEC; ++e) v[e] = fma(beta, (W)in.c[e], v[e]);
     }
   }
-  if (ep.D) store_row<TD, VEC, W>((TD*)ep.D + n * ep.ldd + m, v, valid);
+  if (ep.D) store_row<TD, VEC, W>(pd, v, valid);
 }
 
 }  // namespace plk

@@ -30,6 +30,8 @@ __global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, lon
     if (!GRAD && ep.bias) load_row<T, VEC, W>((const T*)ep.bias + m, bias, valid);
 #pragma unroll(sizeof(T) == 8 ? 1 : 2)
     for (long n = n0 + wave; n < n1; n += 4) {
+      EpilogueInputs<T, TD, GRAD, VEC> in;
+      in.load(ep, (const TD*)ep.C + n * ep.ldc + m, (const T*)ep.Z + n * ep.ldz + m, valid);
       W v[VEC];
       load_row<TP, VEC, W>(P + n * ldP + m, v, valid);
       if constexpr (sizeof(TP) > sizeof(T)) {   // (only 16-bit products come in slices)
@@ -40,7 +42,7 @@ __global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, lon
           for (int e = 0; e < VEC; ++e) v[e] += x[e];
         }
       }
-      apply_epilogue<T, TD, GRAD, VEC>(ep, v, bias, m, n, valid, sums);
+      apply_epilogue<T, TD, GRAD, VEC>(ep, in, v, bias, (TD*)ep.D + n * ep.ldd + m, (T*)ep.preact + n * ep.ldp + m, valid, sums);
     }
   }
   if constexpr (GRAD) {

@@ -1,0 +1,6 @@
+// The 16-bit product (half_product.h) on f16 operands, gradient through an activation.
+#include "kernels/half_product.h"
+
+namespace plk {
+int half_gradient_f16(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epilogue& ep) { return half_direct<f16_t, f16_t, true>(c, plan, at, bt, ep); }
+}  // namespace plk

@@ -53,5 +53,75 @@ int bias_fold(int type, long M, long rows, const void* partial, void* dbias, hip
 long epilogue_pass_rows(int type, long M, long N);
 int epilogue_pass(int type, int type_d, bool grad, long M, long N, const void* P, long ldP, long slice, int slices, const Epilogue& ep, hipStream_t stream);
 
+struct Call {
+  const char* who;
+  int type, type_d;
+  char ta, tb;
+  long M, N, K;
+  double alpha;
+  const void* A; long lda;
+  const void* B; long ldb;
+  Epilogue ep;
+  bool grad;
+  void* dbias;
+  void* workspace; long workspace_bytes;
+  hipStream_t stream;
+};
+
+constexpr int H_BK = 64;   // panel depth of the 16-bit product
+
+// How a 16-bit product is launched: macro tile, and how many ways K is split so that few tiles still fill the chip.  A
+// function of the shape alone (the workspace is sized with it).  The times (microseconds) are fits to products of 256, 512
+// and more workgroups at K = 512 .. 8192: a round of 256 x 256 tiles, one per compute unit, 10 + 0.0222 K (1511 TFLOP/s
+// but for its ends); of 128 x 128 tiles, two per unit, 5 + 0.0136 K, or with one per unit 3 + 0.0105 K; a call 4.  Slices go
+// out in 32 bits and come back through a pass at about 4 TB/s, a launch of its own.
+struct HalfPlan { int tile, splits, kchunk; };   // tile 0: rows of fewer than 8 elements
+inline double half_rounds_us(int tile, long blocks, double k) {
+  if (tile == 256) return (double)((blocks + 255) / 256) * (10.0 + 0.0222 * k);
+  const long rem = blocks % 512;
+  return (double)(blocks / 512) * (5.0 + 0.0136 * k) + (rem == 0 ? 0.0 : rem <= 256 ? 3.0 + 0.0105 * k : 5.0 + 0.0136 * k);
+}
+inline HalfPlan plan_half(bool at, bool bt, long M, long N, long K) {
+  if ((at ? K : M) < 8 || (bt ? N : K) < 8) return {0, 1, 0};
+  HalfPlan best = {128, 1, 0};
+  double best_us = 1e30;
+  for (const int tile : {128, 256}) {
+    const long tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+    for (int s = 1; s <= 32; ++s) {
+      const long kc = ((K + s - 1) / s + H_BK - 1) / H_BK * H_BK;
+      if (s > 1 && (kc < 2 * H_BK || (long)s * M * N * 4 > (256L << 20) || tiles * s > 2048)) break;
+      const long splits = s > 1 ? (K + kc - 1) / kc : 1;
+      if (splits != s) continue;
+      double us = 4.0 + half_rounds_us(tile, tiles * s, s > 1 ? (double)kc : (double)K);
+      if (s > 1) us += 4.0 + (4.0 * s + 4.0) * (double)M * (double)N / 4e6;
+      if (us < best_us * (s > 1 ? 0.95 : 1.0)) best_us = us, best = {tile, s, s > 1 ? (int)kc : 0};
+    }
+  }
+  return best;
+}
+
+// rows of partial bias gradients the 16-bit product leaves: two per tile column, or those of the pass
+inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
+  return p.splits > 1 || p.tile == 0 ? epilogue_pass_rows(type, M, N) : 2 * ((N + p.tile - 1) / p.tile);
+}
+
+// requests: 16-byte granules, and offsets from a panel's first element in 32 bits (256 rows of a K-major operand, 64 k-rows
+// of an MN-major one)
+inline bool in_offset_range(long lda, long ldb) { return lda < (1L << 22) && ldb < (1L << 22); }
+inline bool can_request(const void* A, long lda, const void* B, long ldb) {
+  return aligned_to(A, 16) && aligned_to(B, 16) && lda % 8 == 0 && ldb % 8 == 0 && in_offset_range(lda, ldb);
+}
+
+// The 16-bit product, one source per operand type and kind: D of the operands' type, D in fp32 (and the fp32 slices of a
+// split or thin product), the gradient.
+#define PLK_HALF(T)                                                                                              \
+  int half_forward_##T(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epilogue& ep);               \
+  int half_wide_##T(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epilogue& ep);                  \
+  int half_slices_##T(const Call& c, const HalfPlan& plan, bool at, bool bt, void* slices);                      \
+  int half_gradient_##T(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epilogue& ep);
+PLK_HALF(bf16)
+PLK_HALF(f16)
+#undef PLK_HALF
+
 }  // namespace plk
 #endif
