@@ -23,7 +23,7 @@ namespace plk {
 constexpr int NORM_THREADS = 256;
 constexpr int CHUNK = 8192;          // elements: 16 - 64 KiB, four steps of eight elements a thread
 constexpr int LIST_MAX = 112;        // tensors per launch: 28 bytes each in the kernel's arguments
-constexpr int NORM_BLOCKS = 1024;    // workgroups of one launch at most (four per compute unit), and its partial sums
+constexpr int NORM_BLOCKS = 2048;    // workgroups of one launch at most (eight per compute unit), and its partial sums
 
 struct TensorList {
   const void* src[LIST_MAX];
@@ -116,7 +116,7 @@ template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T*
   }
 }
 
-// partials > 0: every workgroup folds the partial sums of the norm's launches itself, in the same order (8 KiB out of the
+// partials > 0: every workgroup folds the partial sums of the norm's launches itself, in the same order (16 KiB out of the
 // L2 against a launch of its own), and workgroup 0 of the first launch stores the norm.  partials == 0: *norm is given.
 // A factor of exactly 1 leaves tensors that are scaled in place as they are.
 __global__ __launch_bounds__(NORM_THREADS) void grad_scale_kernel(TensorList list, const double* __restrict__ partial, int partials, int store, double max_norm,

@@ -500,10 +500,9 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN * STAGES <= 128 * 128 * 2 ? 2 :
 
 // ---- few columns (single tokens and small batches of them) ----
 // op(A) K-major, op(B) K-major, at most 32 columns: reading A once bounds it, and its latency.  A workgroup owns 16 RB rows
-// of D whole, so there is one launch and no slices: its eight waves split K, each with a ring of D panels of its own in LDS
+// of D whole, so there is one launch and no slices: its WAVES waves split K, each with a ring of D panels of its own in LDS
 // (16 RB rows of A and 16 NB columns of B, 64 deep) that it fills with requests and waits for by itself, without a
 // barrier; 64 KiB of A are in flight per compute unit.  The waves' sums are added in wave order.
-constexpr int FEW_WAVES = 8, FEW_MAX_N = 32;
 
 __device__ __forceinline__ floatx4 mfma16_small(short8_t a, short8_t b, floatx4 c, bf16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -512,13 +511,13 @@ __device__ __forceinline__ floatx4 mfma16_small(short8_t a, short8_t b, floatx4 
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, typename TD, int RB, int NB>
-__global__ __launch_bounds__(FEW_WAVES * 64, 2) void half_few_columns_kernel(int M, int N, int K, const short* __restrict__ A, long lda, const short* __restrict__ B,
+template <typename T, typename TD, int RB, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void half_few_columns_kernel(int M, int N, int K, const short* __restrict__ A, long lda, const short* __restrict__ B,
                                                                              long ldb, Epilogue ep) {
   constexpr int PIECES = 2 * (RB + NB), RING = 16 / PIECES, SLOT = PIECES * 512;   // requests per panel, panels in flight, elements per panel
   constexpr int ROWS = 16 * RB, COLS = 16 * NB, EP_LD = ROWS + 4;
   static_assert(COLS * EP_LD * 2 <= RING * SLOT, "a wave's sums go where its ring was");
-  __shared__ __attribute__((aligned(1024))) short smem[FEW_WAVES * RING * SLOT];
+  __shared__ __attribute__((aligned(1024))) short smem[WAVES * RING * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   short* const mine = smem + wave * RING * SLOT;
   const int m0 = blockIdx.x * ROWS;
@@ -530,7 +529,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 2) void half_few_columns_kernel(int
     const int row = i < 2 * RB ? min(r, M - 1 - m0) : min(r - ROWS, N - 1);
     off[i] = (unsigned)row * (unsigned)(i < 2 * RB ? lda : ldb) * 2u + (unsigned)g * 16u;
   }
-  const int panels = K / H_BK, first = panels * wave / FEW_WAVES, last = panels * (wave + 1) / FEW_WAVES;
+  const int panels = K / H_BK, first = panels * wave / WAVES, last = panels * (wave + 1) / WAVES;
   const short* const Ab = A + (long)m0 * lda;
   auto ask = [&](int p, int slot) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -590,7 +589,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 2) void half_few_columns_kernel(int
     for (int e = 0; e < 8; ++e) v[e] = bias[e] = unused[e] = 0.0f;
     if (ep.bias) load_row<T, 8, float>((const T*)ep.bias + m, bias, valid);
 #pragma unroll
-    for (int w = 0; w < FEW_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float* const q = reinterpret_cast<const float*>(smem + w * RING * SLOT) + n * EP_LD + 8 * sub;
       const floatx4 lo = *reinterpret_cast<const floatx4*>(q), hi = *reinterpret_cast<const floatx4*>(q + 4);
 #pragma unroll
@@ -602,13 +601,21 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 2) void half_few_columns_kernel(int
 
 template <typename T, typename TD>
 int launch_few_columns(long M, long N, long K, const void* A, long lda, const void* B, long ldb, const Epilogue& ep, hipStream_t stream) {
-#define FEW(RB, NB)                                                                                                                                        \
-  hipLaunchKernelGGL((half_few_columns_kernel<T, TD, RB, NB>), dim3((unsigned)((M + 16 * RB - 1) / (16 * RB))), dim3(FEW_WAVES * 64), 0, stream, (int)M, (int)N, \
+#define FEW(RB, NB, WAVES)                                                                                                                                         \
+  hipLaunchKernelGGL((half_few_columns_kernel<T, TD, RB, NB, WAVES>), dim3((unsigned)((M + 16 * RB - 1) / (16 * RB))), dim3(WAVES * 64), 0, stream, (int)M, (int)N, \
                      (int)K, (const short*)A, lda, (const short*)B, ldb, ep)
-  // 32 rows a workgroup where that still fills every compute unit twice: half the reads of B
-  const bool two = M >= 32 * 512;
-  if (N <= 16) { if (two) FEW(2, 1); else FEW(1, 1); }
-  else { if (two) FEW(2, 2); else FEW(1, 2); }
+  // One workgroup of eight waves per compute unit up to 256 of them; more come in fours, two to a unit, so that one's first
+  // requests and its sums overlap the other's stream; 32 rows each where that still gives every unit two: half the reads of B.
+  const long blocks = (M + 15) / 16;
+#define FEW_COLUMNS(NB)                  \
+  do {                                   \
+    if (blocks <= 256) FEW(1, NB, 8);    \
+    else if (blocks < 1024) FEW(1, NB, 4); \
+    else FEW(2, NB, 4);                  \
+  } while (0)
+  if (N <= 16) FEW_COLUMNS(1);
+  else FEW_COLUMNS(2);
+#undef FEW_COLUMNS
 #undef FEW
   return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
 }
@@ -654,9 +661,7 @@ int launch_half(const HalfPlan& plan, bool at, bool bt, long M, long N, long K, 
 template <typename T, typename TD, bool GRAD>
 int half_direct(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epilogue& ep) {
   if constexpr (!GRAD) {
-    // few columns: the requests' alignment, whole panels
-    if (at && !bt && c.N <= FEW_MAX_N && c.K > 0 && c.K % H_BK == 0 && can_request(c.A, c.lda, c.B, c.ldb))
-      return launch_few_columns<T, TD>(c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
+    if (few_columns(c, at, bt)) return launch_few_columns<T, TD>(c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
   }
   return launch_half<T, TD, GRAD>(plan, at, bt, c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
 }

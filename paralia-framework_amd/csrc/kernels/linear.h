@@ -73,13 +73,13 @@ constexpr int H_BK = 64;   // panel depth of the 16-bit product
 // How a 16-bit product is launched: macro tile, and how many ways K is split so that few tiles still fill the chip.  A
 // function of the shape alone (the workspace is sized with it).  The times (microseconds) are fits to products of 256, 512
 // and more workgroups at K = 512 .. 8192: a round of 256 x 256 tiles, one per compute unit, 10 + 0.0222 K (1511 TFLOP/s
-// but for its ends); of 128 x 128 tiles, two per unit, 5 + 0.0136 K, or with one per unit 3 + 0.0105 K; a call 4.  Slices go
+// but for its ends); of 128 x 128 tiles, two per unit, 5 + 0.0136 K, or with one per unit 3.5 + 0.0069 K; a call 4.  Slices go
 // out in 32 bits and come back through a pass at about 4 TB/s, a launch of its own.
 struct HalfPlan { int tile, splits, kchunk; };   // tile 0: rows of fewer than 8 elements
 inline double half_rounds_us(int tile, long blocks, double k) {
   if (tile == 256) return (double)((blocks + 255) / 256) * (10.0 + 0.0222 * k);
   const long rem = blocks % 512;
-  return (double)(blocks / 512) * (5.0 + 0.0136 * k) + (rem == 0 ? 0.0 : rem <= 256 ? 3.0 + 0.0105 * k : 5.0 + 0.0136 * k);
+  return (double)(blocks / 512) * (5.0 + 0.0136 * k) + (rem == 0 ? 0.0 : rem <= 256 ? 3.5 + 0.0069 * k : 5.0 + 0.0136 * k);
 }
 inline HalfPlan plan_half(bool at, bool bt, long M, long N, long K) {
   if ((at ? K : M) < 8 || (bt ? N : K) < 8) return {0, 1, 0};
@@ -110,6 +110,12 @@ inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
 inline bool in_offset_range(long lda, long ldb) { return lda < (1L << 22) && ldb < (1L << 22); }
 inline bool can_request(const void* A, long lda, const void* B, long ldb) {
   return aligned_to(A, 16) && aligned_to(B, 16) && lda % 8 == 0 && ldb % 8 == 0 && in_offset_range(lda, ldb);
+}
+
+// few columns of two K-major operands that can be requested, in whole panels of k: a kernel of their own
+constexpr int FEW_MAX_N = 32;
+inline bool few_columns(const Call& c, bool at, bool bt) {
+  return at && !bt && !c.grad && c.N <= FEW_MAX_N && c.K > 0 && c.K % H_BK == 0 && can_request(c.A, c.lda, c.B, c.ldb);
 }
 
 // The 16-bit product, one source per operand type and kind: D of the operands' type, D in fp32 (and the fp32 slices of a
