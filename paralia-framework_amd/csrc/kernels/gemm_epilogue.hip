@@ -9,22 +9,54 @@
 namespace plk {
 
 // The workspace of one call, in the order it is laid out: what the product needs, the product itself (fp32 and fp64
-// operands), the partial bias gradients.
-struct Workspace { long product_ws, product, partial; long bytes() const { return product_ws + product + partial; } };
+// operands), the partial bias gradients, aligned copies of 16-bit operands.
+struct Workspace { long product_ws, product, partial, copies; long bytes() const { return product_ws + product + partial + copies; } };
 inline long round16(long b) { return (b + 15) & ~15L; }
 inline Workspace workspace_for(int type, bool at, bool bt, long M, long N, long K, bool dbias) {
-  Workspace w = {0, 0, 0};
+  Workspace w = {0, 0, 0, 0};
   const long wide = type == PL_TYPE_F64 ? 8 : 4;
   if (type_size(type) == 2) {
     const HalfPlan p = plan_half(at, bt, M, N, K);
     if (p.splits > 1 || p.tile == 0) w.product = round16((long)p.splits * M * N * 4);
     if (dbias) w.partial = round16(half_partial_rows({p.tile == 256 ? 128 : p.tile, p.splits, 0}, type, M, N) * M * wide);   // (unaligned operands: the small tile)
+    w.copies = half_copies(at, bt, M, N, K).bytes();
   } else {
     w.product_ws = round16(pl_gemm_tile_alone_workspace_bytes(at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, type_size(type)));
     w.product = round16(M * N * wide);
     if (dbias) w.partial = round16(epilogue_pass_rows(type, M, N) * M * wide);
   }
   return w;
+}
+
+// blockIdx.y: which operand.  `rows` rows of `extent` elements into `rows_to` rows of ld_to, zeros behind them.
+struct HalfCopyJob { const short* from; short* to; long ld, ld_to, rows, rows_to; int extent; };
+__global__ __launch_bounds__(256) void half_copy_kernel(HalfCopyJob a, HalfCopyJob b) {
+  const HalfCopyJob j = blockIdx.y == 0 ? a : b;
+  const long per_row = j.ld_to / 8, total = per_row * j.rows_to;
+  typedef Loose<short>::vec vec;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const long row = i / per_row;
+    const int at = (int)(i - row * per_row) * 8, left = row < j.rows ? j.extent - at : 0;
+    const short* const p = j.from + row * j.ld + at;
+    vec v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (left >= 8) {
+      v = *reinterpret_cast<const Loose<short>::type*>(p);
+    } else if (left > 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p[e < left ? e : left - 1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < left ? v[e] : (short)0;
+    }
+    *reinterpret_cast<vec*>(j.to + row * j.ld_to + at) = v;
+  }
+}
+int half_copy(const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const HalfCopies& to) {
+  const HalfCopyJob a = {(const short*)A, (short*)copy_a, lda, to.ld_a, at ? c.M : c.K, to.bytes_a / (2 * to.ld_a), (int)(at ? c.K : c.M)};
+  const HalfCopyJob b = {(const short*)B, (short*)copy_b, ldb, to.ld_b, bt ? c.K : c.N, to.bytes_b / (2 * to.ld_b), (int)(bt ? c.N : c.K)};
+  const long most = (to.bytes_a > to.bytes_b ? to.bytes_a : to.bytes_b) / 16;
+  const long blocks = (most + 255) / 256;
+  hipLaunchKernelGGL(half_copy_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), 0, c.stream, a, b);
+  return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
 }
 
 int run_product(Call& c) {
@@ -70,6 +102,16 @@ int run_product(Call& c) {
   if (es == 2) {
     HalfPlan plan = plan_half(at, bt, M, N, K);
     if (empty) plan.splits = 1, plan.kchunk = 0;
+    const HalfCopies copies = half_copies(at, bt, M, N, K);
+    if (!empty && copies.bytes() > 0 && !can_request(c.A, c.lda, c.B, c.ldb) && in_offset_range(copies.ld_a, copies.ld_b)) {
+      char* const copy_a = ws + w.product_ws + w.product + w.partial;
+      rc_ = half_copy(c.A, c.lda, copy_a, c.B, c.ldb, copy_a + copies.bytes_a, c, at, bt, copies);
+      if (rc_ != PL_OK) return rc_;
+      c.A = copy_a, c.lda = copies.ld_a;
+      c.B = copy_a + copies.bytes_a, c.ldb = copies.ld_b;
+      c.K = (K + H_BK - 1) / H_BK * H_BK;
+      c.padded = true;
+    }
     if (plan.tile == 256 && !can_request(c.A, c.lda, c.B, c.ldb)) plan.tile = 128;
     rows = half_partial_rows(plan, c.type, M, N);
     const bool f16 = c.type == PL_TYPE_F16, sliced = (plan.tile == 0 || plan.splits > 1) && !few_columns(c, at, bt);

@@ -199,7 +199,7 @@ template <bool KMAJOR, int EXT> struct Reader {
   }
 };
 
-// fast: 2: both operands can be requested, 1: leading dimensions within the offsets' range, 0: neither.  kchunk: split K (0: no).
+// fast: 3: both operands can be requested and their rows read to a multiple of 8 elements, 2: requested, 1: leading dimensions within the offsets' range, 0: neither.  kchunk: split K (0: no).
 template <typename T, typename TD, bool AK, bool BKM, int BM, int BN, int STAGES, bool GRAD>
 __global__ __launch_bounds__(H_THREADS, (BM * BN * STAGES <= 128 * 128 * 2 ? 2 : 1)) void half_product_kernel(int M, int N, int K, const short* __restrict__ A, long lda,
                                                                                                const short* __restrict__ B, long ldb, int gm, int gn, int fast,
@@ -266,8 +266,8 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN * STAGES <= 128 * 128 * 2 ? 2 :
   // Whole panels that the requests may load.  The last granule of an MN-major row at the edge of the matrix reaches past
   // it where the extent is not a multiple of 8; behind every k-row but the last that is still the operand's own memory
   // (its leading dimension is a multiple of 8), so the last k-row is left to the guarded step.
-  const bool last_row_guarded = (!AK && mrem < BM && (M & 7)) || (!BKM && nrem < BN && (N & 7));
-  const int nfull = fast == 2 ? (K - (last_row_guarded ? 1 : 0)) / H_BK : 0;
+  const bool last_row_guarded = fast < 3 && ((!AK && mrem < BM && (M & 7)) || (!BKM && nrem < BN && (N & 7)));
+  const int nfull = fast >= 2 ? (K - (last_row_guarded ? 1 : 0)) / H_BK : 0;
   if (nfull > 0) {
     unsigned oa[PA::NV], ob[PB::NV];
     request_offsets<PA, AK>(oa, lda, mrem, wave, lane);
@@ -637,9 +637,9 @@ __global__ __launch_bounds__(256) void half_thin_kernel(long M, long N, int K, c
 }
 
 template <typename T, typename TD, bool GRAD>
-int launch_half(const HalfPlan& plan, bool at, bool bt, long M, long N, long K, const void* A, long lda, const void* B, long ldb, const Epilogue& ep, hipStream_t stream) {
+int launch_half(const HalfPlan& plan, bool at, bool bt, bool padded, long M, long N, long K, const void* A, long lda, const void* B, long ldb, const Epilogue& ep, hipStream_t stream) {
   const int gm = (int)((M + plan.tile - 1) / plan.tile), gn = (int)((N + plan.tile - 1) / plan.tile);
-  const int fast = can_request(A, lda, B, ldb) ? 2 : in_offset_range(lda, ldb) ? 1 : 0;
+  const int fast = padded ? 3 : can_request(A, lda, B, ldb) ? 2 : in_offset_range(lda, ldb) ? 1 : 0;
 #define HALF(AKF, BKF, TILE, STAGES)                                                                                                                     \
   hipLaunchKernelGGL((half_product_kernel<T, TD, AKF, BKF, TILE, TILE, STAGES, GRAD>), dim3(gm * gn, plan.splits), dim3(H_THREADS), 0, stream, (int)M, (int)N, \
                      (int)K, (const short*)A, lda, (const short*)B, ldb, gm, gn, fast, plan.kchunk, ep)
@@ -651,7 +651,7 @@ int launch_half(const HalfPlan& plan, bool at, bool bt, long M, long N, long K, 
     else HALF(false, false, TILE, STAGES);         \
   } while (0)
   if (plan.tile == 256) HALF_TILE(256, 2);
-  else if (fast == 2 && (long)gm * gn * plan.splits <= 256) HALF_TILE(128, 4);
+  else if (fast >= 2 && (long)gm * gn * plan.splits <= 256) HALF_TILE(128, 4);
   else HALF_TILE(128, 2);
 #undef HALF_TILE
 #undef HALF
@@ -663,7 +663,7 @@ int half_direct(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epi
   if constexpr (!GRAD) {
     if (few_columns(c, at, bt)) return launch_few_columns<T, TD>(c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
   }
-  return launch_half<T, TD, GRAD>(plan, at, bt, c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
+  return launch_half<T, TD, GRAD>(plan, at, bt, c.padded, c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, ep, c.stream);
 }
 
 // The product alone, as fp32 slices for the pass to add and finish.
@@ -678,7 +678,7 @@ template <typename T> int half_slices(const Call& c, const HalfPlan& plan, bool 
   plain.alpha = 1.0;
   plain.D = slices;
   plain.ldd = c.M;
-  return launch_half<T, float, false>(plan, at, bt, c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, plain, c.stream);
+  return launch_half<T, float, false>(plan, at, bt, c.padded, c.M, c.N, c.K, c.A, c.lda, c.B, c.ldb, plain, c.stream);
 }
 
 }  // namespace plk

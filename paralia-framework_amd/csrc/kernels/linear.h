@@ -63,6 +63,7 @@ struct Call {
   const void* B; long ldb;
   Epilogue ep;
   bool grad;
+  bool padded;           // 16-bit operands with whole panels of k, whose rows may be read to a multiple of 64 elements
   void* dbias;
   void* workspace; long workspace_bytes;
   hipStream_t stream;
@@ -111,6 +112,29 @@ inline bool in_offset_range(long lda, long ldb) { return lda < (1L << 22) && ldb
 inline bool can_request(const void* A, long lda, const void* B, long ldb) {
   return aligned_to(A, 16) && aligned_to(B, 16) && lda % 8 == 0 && ldb % 8 == 0 && in_offset_range(lda, ldb);
 }
+
+// Operands that cannot be requested are multiplied from aligned copies where that pays: a panel of unaligned 16-byte loads
+// takes a compute unit 0.7 - 1.1 us longer than a requested one (misaligned lanes are served one by one), each operand's
+// panels are loaded by every tile in its row or column, and the copies cost one launch and one pass over the operands
+// (4100 x 1023 x 2052, rows of an odd number of elements: 70 -> @ us).  The space is set aside by the shape alone: where a
+// contiguous extent is no multiple of 8, so that dense operands could not be aligned.
+struct HalfCopies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
+inline HalfCopies half_copies(bool at, bool bt, long M, long N, long K) {
+  const long ext_a = at ? K : M, rows_a = at ? M : K, ext_b = bt ? N : K, rows_b = bt ? K : N;
+  HalfCopies c = {0, 0, 0, 0};
+  if ((ext_a % 8 == 0 && ext_b % 8 == 0) || ext_a < 8 || ext_b < 8) return c;
+  const double tiles = (double)((M + 127) / 128) * (double)((N + 127) / 128);
+  const double slow_us = 0.8 * (double)(K / H_BK) * (tiles > 256.0 ? tiles / 256.0 : 1.0), copy_us = 6.0 + 4.0 * (double)K * (double)(M + N) / 3e6;
+  if (slow_us < copy_us) return c;
+  // rows in whole cache lines, and k filled up with zeros to whole panels in either layout
+  auto whole = [](long n) { return (n + H_BK - 1) / H_BK * H_BK; };
+  c.ld_a = whole(ext_a);
+  c.ld_b = whole(ext_b);
+  c.bytes_a = (at ? rows_a : whole(rows_a)) * c.ld_a * 2;
+  c.bytes_b = (bt ? whole(rows_b) : rows_b) * c.ld_b * 2;
+  return c;
+}
+int half_copy(const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const HalfCopies& to);
 
 // few columns of two K-major operands that can be requested, in whole panels of k: a kernel of their own
 constexpr int FEW_MAX_N = 32;
