@@ -32,14 +32,16 @@ template <typename T> struct Loose {
 // (What is read or written once goes past the caches, non-temporal: 16384 x 8192 x 4096 with the gradient 1017 -> 967 us, the
 // panels of the product keep the L2 to themselves.)
 // N consecutive elements, `valid` of which are inside the matrix (the others read as zero and are not written).
-template <typename T, int N, typename W>
+template <typename T, int N, typename W, bool ONCE = false>
 __device__ __forceinline__ void load_row(const T* p, W (&v)[N], int valid) {
   constexpr int V = Loose<T>::N;
   static_assert(N % V == 0, "whole vectors");
   if (valid >= N) {
 #pragma unroll
     for (int q = 0; q < N / V; ++q) {
-      const typename Loose<T>::vec x = *reinterpret_cast<const typename Loose<T>::type*>(p + q * V);
+      typename Loose<T>::vec x;
+      if constexpr (ONCE) x = __builtin_nontemporal_load(reinterpret_cast<const typename Loose<T>::type*>(p + q * V));
+      else x = *reinterpret_cast<const typename Loose<T>::type*>(p + q * V);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[q * V + e] = (W)x[e];
     }

@@ -22,7 +22,7 @@ namespace plk {
 
 constexpr int NORM_THREADS = 256;
 constexpr int CHUNK = 8192;          // elements: 16 - 64 KiB, four steps of eight elements a thread
-constexpr int LIST_MAX = 112;        // tensors per launch: 28 bytes each in the kernel's arguments
+constexpr int LIST_MAX = 128;        // tensors per launch: two per lane, 28 bytes each in the kernel's arguments
 constexpr int NORM_BLOCKS = 2048;    // workgroups of one launch at most (eight per compute unit), and its partial sums
 
 struct TensorList {
@@ -32,16 +32,37 @@ struct TensorList {
   unsigned first[LIST_MAX + 1];      // the list's chunk at which each tensor starts; then the number of chunks
   int n;
 };
+static_assert(sizeof(TensorList) <= 4096 - 64, "the list and what goes with it are kernel arguments");
 
-__device__ __forceinline__ int tensor_of(const TensorList& list, unsigned chunk) {
-  int lo = 0, hi = list.n - 1;       // the last tensor that starts at or before the chunk (empty tensors start where the next does)
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (list.first[mid] <= chunk) lo = mid;
-    else hi = mid - 1;
+// The list in registers: lane l holds tensors l and l + 64, fetched all at once (a search through the kernel's arguments is
+// seven dependent fetches, 3 us of a small call).  The tensor of a chunk is the number of tensors that start at or before
+// it; what the list says of it then comes out of that lane.
+struct ListLanes {
+  unsigned long long src[2], dst[2], count_type[2];
+  unsigned first[2];
+  __device__ __forceinline__ explicit ListLanes(const TensorList& list, bool with_dst) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = (int)(threadIdx.x & 63) + 64 * h, j = i < list.n ? i : list.n - 1;
+      first[h] = i < list.n ? list.first[j] : 0xffffffffu;
+      src[h] = (unsigned long long)list.src[j];
+      dst[h] = with_dst ? (unsigned long long)list.dst[j] : 0;
+      count_type[h] = (unsigned long long)list.count_type[j];
+    }
   }
-  return lo;
-}
+  static __device__ __forceinline__ unsigned pick(unsigned v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  static __device__ __forceinline__ unsigned long long pick(unsigned long long v, int lane) {
+    return ((unsigned long long)pick((unsigned)(v >> 32), lane) << 32) | pick((unsigned)v, lane);
+  }
+  struct Chunk { const void* src; void* dst; long long at; int count, type; };
+  __device__ __forceinline__ Chunk chunk(unsigned c) const {
+    const int t = __popcll(__ballot(first[0] <= c)) + __popcll(__ballot(first[1] <= c)) - 1;
+    const int h = t >> 6, lane = t & 63;
+    const unsigned long long ct = pick(h ? count_type[1] : count_type[0], lane);
+    const long long at = (long long)(c - pick(h ? first[1] : first[0], lane)) * CHUNK, left = (long long)(ct >> 2) - at;
+    return {(const void*)pick(h ? src[1] : src[0], lane), (void*)pick(h ? dst[1] : dst[0], lane), at, left < CHUNK ? (int)left : CHUNK, (int)(ct & 3)};
+  }
+};
 
 __device__ __forceinline__ double sum_block(double v) {
   __shared__ double part[NORM_THREADS / 64];
@@ -73,16 +94,15 @@ template <typename T> __device__ __forceinline__ double chunk_squares(const T* _
 
 __global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(TensorList list, double* __restrict__ partial) {
   const unsigned chunks = list.first[list.n];
+  const ListLanes lanes(list, false);
   double acc = 0.0;
   for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int t = tensor_of(list, c);
-    const long long ct = list.count_type[t], at = (long long)(c - list.first[t]) * CHUNK, left = (ct >> 2) - at;
-    const int count = left < CHUNK ? (int)left : CHUNK;
-    switch ((int)(ct & 3)) {
-      case PL_TYPE_F64: acc += chunk_squares((const double*)list.src[t] + at, count); break;
-      case PL_TYPE_F32: acc += chunk_squares((const float*)list.src[t] + at, count); break;
-      case PL_TYPE_F16: acc += chunk_squares((const f16_t*)list.src[t] + at, count); break;
-      default: acc += chunk_squares((const bf16_t*)list.src[t] + at, count); break;
+    const ListLanes::Chunk k = lanes.chunk(c);
+    switch (k.type) {
+      case PL_TYPE_F64: acc += chunk_squares((const double*)k.src + k.at, k.count); break;
+      case PL_TYPE_F32: acc += chunk_squares((const float*)k.src + k.at, k.count); break;
+      case PL_TYPE_F16: acc += chunk_squares((const f16_t*)k.src + k.at, k.count); break;
+      default: acc += chunk_squares((const bf16_t*)k.src + k.at, k.count); break;
     }
   }
   acc = sum_block(acc);
@@ -108,7 +128,7 @@ template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T*
     const int valid = count - at;
     if (valid > 0) {
       wide_t<T> v[8];
-      load_row<T, 8, wide_t<T>>(p + at, v, valid);
+      load_row<T, 8, wide_t<T>, true>(p + at, v, valid);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= f;
       store_row<T, 8, wide_t<T>>(q + at, v, valid);
@@ -121,23 +141,21 @@ template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T*
 // A factor of exactly 1 leaves tensors that are scaled in place as they are.
 __global__ __launch_bounds__(NORM_THREADS) void grad_scale_kernel(TensorList list, const double* __restrict__ partial, int partials, int store, double max_norm,
                                                                  double eps, double* norm) {
+  const ListLanes lanes(list, true);
+  const unsigned chunks = list.first[list.n];
   const double total = partials > 0 ? fold_norm(partial, partials) : *norm;
   if (partials > 0 && store && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
   const double ratio = max_norm / (total + eps);
   const double scale = ratio > 1.0 ? 1.0 : ratio;   // (a NaN stays a NaN)
-  const unsigned chunks = list.first[list.n];
   // last chunk first: what the norm read last is what the caches still hold
   for (unsigned r = blockIdx.x; r < chunks; r += gridDim.x) {
-    const unsigned c = chunks - 1 - r;
-    const int t = tensor_of(list, c);
-    const long long ct = list.count_type[t], at = (long long)(c - list.first[t]) * CHUNK, left = (ct >> 2) - at;
-    const int count = left < CHUNK ? (int)left : CHUNK;
-    if (scale == 1.0 && list.src[t] == list.dst[t]) continue;
-    switch ((int)(ct & 3)) {
-      case PL_TYPE_F64: chunk_scale((const double*)list.src[t] + at, (double*)list.dst[t] + at, count, scale); break;
-      case PL_TYPE_F32: chunk_scale((const float*)list.src[t] + at, (float*)list.dst[t] + at, count, scale); break;
-      case PL_TYPE_F16: chunk_scale((const f16_t*)list.src[t] + at, (f16_t*)list.dst[t] + at, count, scale); break;
-      default: chunk_scale((const bf16_t*)list.src[t] + at, (bf16_t*)list.dst[t] + at, count, scale); break;
+    const ListLanes::Chunk k = lanes.chunk(chunks - 1 - r);
+    if (scale == 1.0 && k.src == k.dst) continue;
+    switch (k.type) {
+      case PL_TYPE_F64: chunk_scale((const double*)k.src + k.at, (double*)k.dst + k.at, k.count, scale); break;
+      case PL_TYPE_F32: chunk_scale((const float*)k.src + k.at, (float*)k.dst + k.at, k.count, scale); break;
+      case PL_TYPE_F16: chunk_scale((const f16_t*)k.src + k.at, (f16_t*)k.dst + k.at, k.count, scale); break;
+      default: chunk_scale((const bf16_t*)k.src + k.at, (bf16_t*)k.dst + k.at, k.count, scale); break;
     }
   }
 }
