@@ -14,7 +14,7 @@ constexpr int PASS_THREADS = 256;
 
 // v(m, n) <- sum over slices of P(m, n), through the epilogue.  blockIdx.x: 64 * VEC rows, blockIdx.y: a range of `per`
 // columns.  GRAD with ep.partial: row blockIdx.y of the partial sums.
-template <typename TP, typename T, typename TD, bool GRAD, int VEC>
+template <typename TP, typename T, typename TD, bool GRAD, bool SLICES, int VEC>
 __global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, long N, long per, const TP* __restrict__ P, long ldP, long slice, int slices,
                                                                     Epilogue ep) {
   using W = wide_t<T>;
@@ -34,7 +34,7 @@ __global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, lon
       in.load(ep, (const TD*)ep.C + n * ep.ldc + m, (const T*)ep.Z + n * ep.ldz + m, valid);
       W v[VEC];
       load_row<TP, VEC, W>(P + n * ldP + m, v, valid);
-      if constexpr (sizeof(TP) > sizeof(T)) {   // (only 16-bit products come in slices)
+      if constexpr (SLICES) {
         for (int s = 1; s < slices; ++s) {
           W x[VEC];
           load_row<TP, VEC, W>(P + s * slice + n * ldP + m, x, valid);
@@ -102,7 +102,16 @@ int launch_epilogue_pass(long M, long N, const TP* P, long ldP, long slice, int 
   constexpr int VEC = pass_vec<T>();
   const long ranges = pass_ranges<T>(M, N), per = (N + ranges - 1) / ranges;
   const dim3 grid((unsigned)((M + 64 * VEC - 1) / (64 * VEC)), (unsigned)((N + per - 1) / per));
-hipLaunchKernelGGL((epilogue_pass_kernel<TP, T, TD, GRAD, VEC>), grid, dim3(PASS_THREADS), 0, stream, M, N, per, P, ldP, slice, slices, ep);
+#define LAUNCH(SLICES) \
+  hipLaunchKernelGGL((epilogue_pass_kernel<TP, T, TD, GRAD, SLICES, VEC>), grid, dim3(PASS_THREADS), 0, stream, M, N, per, P, ldP, slice, slices, ep)
+  // (a 16-bit operand is no slice of a product; the fp64 gradient has no scalar registers left for slices)
+  if constexpr (sizeof(TP) == sizeof(wide_t<T>) && !(GRAD && sizeof(T) == 8)) {
+    if (slices > 1) LAUNCH(true);
+    else LAUNCH(false);
+  } else {
+    LAUNCH(false);
+  }
+#undef LAUNCH
   return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
 }
 

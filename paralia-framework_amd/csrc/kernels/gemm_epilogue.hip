@@ -8,12 +8,11 @@
 
 namespace plk {
 
-// The workspace of one call, in the order it is laid out: what the product needs, the product itself (fp32 and fp64
-// operands), the partial bias gradients, aligned copies of 16-bit operands.
-struct Workspace { long product_ws, product, partial, copies; long bytes() const { return product_ws + product + partial + copies; } };
+// The workspace of one call, in the order it is laid out: the product or its slices, the partial bias gradients, aligned copies of 16-bit operands.
+struct Workspace { long product, partial, copies; long bytes() const { return product + partial + copies; } };
 inline long round16(long b) { return (b + 15) & ~15L; }
 inline Workspace workspace_for(int type, bool at, bool bt, long M, long N, long K, bool dbias) {
-  Workspace w = {0, 0, 0, 0};
+  Workspace w = {0, 0, 0};
   const long wide = type == PL_TYPE_F64 ? 8 : 4;
   if (type_size(type) == 2) {
     const HalfPlan p = plan_half(at, bt, M, N, K);
@@ -21,8 +20,8 @@ inline Workspace workspace_for(int type, bool at, bool bt, long M, long N, long 
     if (dbias) w.partial = round16(half_partial_rows({p.tile == 256 ? 128 : p.tile, p.splits, 0}, type, M, N) * M * wide);   // (unaligned operands: the small tile)
     w.copies = half_copies(at, bt, M, N, K).bytes();
   } else {
-    w.product_ws = round16(pl_gemm_tile_alone_workspace_bytes(at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, type_size(type)));
-    w.product = round16(M * N * wide);
+    // the slices of a product alone on the device, or the product and behind it the slices of its tail
+    w.product = round16(M * N * wide) + round16(pl_gemm_tile_alone_workspace_bytes(at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, type_size(type)));
     if (dbias) w.partial = round16(epilogue_pass_rows(type, M, N) * M * wide);
   }
   return w;
@@ -57,6 +56,10 @@ int half_copy(const void* A, long lda, void* copy_a, const void* B, long ldb, vo
   const long blocks = (most + 255) / 256;
   hipLaunchKernelGGL(half_copy_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), 0, c.stream, a, b);
   return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
+}
+
+bool plain_product(const Call& c) {
+  return !c.grad && c.ep.act == PL_ACT_NONE && !c.ep.bias && !c.ep.preact && (c.ep.beta == 0.0 || c.ep.C == c.ep.D);
 }
 
 int run_product(Call& c) {
@@ -95,7 +98,7 @@ int run_product(Call& c) {
   if (w.bytes() > 0 && (!c.workspace || !aligned_to(c.workspace, 16) || c.workspace_bytes < w.bytes())) return refuse(PL_ERR_ARG, who, "workspace null, too small or not 16-byte aligned");
   char* const ws = (char*)c.workspace;
   ep.alpha = empty ? 0.0 : c.alpha;
-  ep.partial = c.dbias ? ws + w.product_ws + w.product : nullptr;
+  ep.partial = c.dbias ? ws + w.product : nullptr;
   if (empty) c.K = 0;
   int rc_;
   long rows;
@@ -104,7 +107,7 @@ int run_product(Call& c) {
     if (empty) plan.splits = 1, plan.kchunk = 0;
     const HalfCopies copies = half_copies(at, bt, M, N, K);
     if (!empty && copies.bytes() > 0 && !can_request(c.A, c.lda, c.B, c.ldb) && in_offset_range(copies.ld_a, copies.ld_b)) {
-      char* const copy_a = ws + w.product_ws + w.product + w.partial;
+      char* const copy_a = ws + w.product + w.partial;
       rc_ = half_copy(c.A, c.lda, copy_a, c.B, c.ldb, copy_a + copies.bytes_a, c, at, bt, copies);
       if (rc_ != PL_OK) return rc_;
       c.A = copy_a, c.lda = copies.ld_a;
@@ -126,13 +129,16 @@ int run_product(Call& c) {
       rc_ = f16 ? half_forward_f16(c, plan, at, bt, ep) : half_forward_bf16(c, plan, at, bt, ep);
     }
   } else {
-    void* const product = ws + w.product_ws;
     rows = epilogue_pass_rows(c.type, M, N);
-    if (c.type == PL_TYPE_F64)
-      rc_ = pl_dgemm_tile_alone(c.ta, c.tb, M, N, c.K, 1.0, (const double*)c.A, c.lda, (const double*)c.B, c.ldb, 0.0, (double*)product, M, ws, w.product_ws, c.stream);
-    else
-      rc_ = pl_sgemm_tile_alone(c.ta, c.tb, M, N, c.K, 1.0f, (const float*)c.A, c.lda, (const float*)c.B, c.ldb, 0.0f, (float*)product, M, ws, w.product_ws, c.stream);
-    if (rc_ == PL_OK) rc_ = epilogue_pass(c.type, c.type_d, c.grad, M, N, product, M, 0, 1, ep, c.stream);
+    const bool f64 = c.type == PL_TYPE_F64;
+    if (plain_product(c)) {
+      // nothing but the product (and C where D is): the tile GEMM's own epilogue
+      return f64 ? pl_dgemm_tile_alone(c.ta, c.tb, M, N, c.K, ep.alpha, (const double*)c.A, c.lda, (const double*)c.B, c.ldb, ep.beta, (double*)ep.D, ep.ldd, ws, w.product, c.stream)
+                 : pl_sgemm_tile_alone(c.ta, c.tb, M, N, c.K, (float)ep.alpha, (const float*)c.A, c.lda, (const float*)c.B, c.ldb, (float)ep.beta, (float*)ep.D, ep.ldd, ws, w.product, c.stream);
+    }
+    int slices = 1;
+    rc_ = (f64 ? product_slices_f64 : product_slices_f32)(c.ta, c.tb, M, N, c.K, c.A, c.lda, c.B, c.ldb, ws, w.product, f64 && c.grad, &slices, c.stream);
+    if (rc_ == PL_OK) rc_ = epilogue_pass(c.type, c.type_d, c.grad, M, N, ws, M, M * N, slices, ep, c.stream);
   }
   if (rc_ != PL_OK || !c.dbias) return rc_;
   return bias_fold(c.type, M, rows, ep.partial, c.dbias, c.stream);

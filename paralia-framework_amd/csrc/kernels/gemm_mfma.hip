@@ -1140,7 +1140,7 @@ TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero
 template <typename T>
 int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, long lda, const T* B, long ldb, T beta,
                 T* C, long ldc, hipStream_t stream, T* workspace = nullptr, long workspace_bytes = 0, int want_splits = 0,
-                bool alone = false, long m_read = 0, long n_read = 0, bool small_only = false) {
+                bool alone = false, long m_read = 0, long n_read = 0, bool small_only = false, bool leave_slices = false) {
   using Tr = Traits<T>;
   const bool at = (ta == 'T' || ta == 't'), an = (ta == 'N' || ta == 'n');
   const bool bt = (tb == 'T' || tb == 't'), bnn = (tb == 'N' || tb == 'n');
@@ -1221,12 +1221,31 @@ int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, l
   else PLK_LAUNCH(true, false);
 #undef PLK_LAUNCH_T
 #undef PLK_LAUNCH
-  if (splits > 1) {
+  if (splits > 1 && !leave_slices) {
     const long total = M * N;
     const int blocks = (int)((total + 255) / 256 < 8192 ? (total + 255) / 256 : 8192);
     hipLaunchKernelGGL(splitk_reduce_kernel<T>, dim3(blocks), dim3(256), 0, stream, (int)M, (int)N, splits, alpha, workspace, beta, C, ldc);
   }
   return hipGetLastError() == hipSuccess ? 0 : 4;
+}
+
+// For a caller that finishes the product itself (the fused epilogue of the linear layers): op(A) * op(B) as a product alone
+// on the device would run it, into `slices` dense M x N slices at ws that are still to be added (1, or add: the product itself).
+template <typename T>
+int product_slices(char ta, char tb, long M, long N, long K, const T* A, long lda, const T* B, long ldb, T* ws, long ws_bytes, bool add, int* slices, hipStream_t stream) {
+  const bool an = ta == 'N' || ta == 'n', bnn = tb == 'N' || tb == 'n';
+  *slices = K > 0 ? choose_tile<T>(an, bnn, M, N, K, true, true, ws_bytes, true, 0, true).splits : 1;
+  if (add) *slices = 1;
+  if (*slices > 1) return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, ws, ws_bytes, *slices, false, 0, 0, false, true);
+  // one launch, or an unsplit head and a split tail whose slices lie behind the product
+  const long product = (M * N * (long)sizeof(T) + 15) & ~15L;
+  return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, (T*)((char*)ws + product), ws_bytes - product, 0, true);
+}
+int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream) {
+  return product_slices<float>(ta, tb, M, N, K, (const float*)A, lda, (const float*)B, ldb, (float*)ws, ws_bytes, add, slices, stream);
+}
+int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream) {
+  return product_slices<double>(ta, tb, M, N, K, (const double*)A, lda, (const double*)B, ldb, (double*)ws, ws_bytes, add, slices, stream);
 }
 
 template <typename T>

@@ -48,6 +48,10 @@ inline bool same_or_apart(const Range& a, const Range& b) {
   return (a.p == b.p && (a.ld == b.ld || a.cols == 1) && a.size == b.size) || !overlap(a, b);
 }
 
+// gemm_mfma.hip: the fp32 / fp64 product in slices that are still to be added
+int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream);
+int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream);
+
 // epilogue.hip
 int bias_fold(int type, long M, long rows, const void* partial, void* dbias, hipStream_t stream);
 long epilogue_pass_rows(int type, long M, long N);
