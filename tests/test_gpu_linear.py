@@ -1,5 +1,6 @@
 """pl_gemm_epilogue, pl_gemm_epilogue_grad and pl_bias_act_grad on the GPU, against their definitions in 64 bits."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -282,3 +283,292 @@ def test_results_repeat_bit_for_bit(pkg, L):
     for _ in range(3):
         again = product_grad(pkg, L, "bf16", "N", "N", opA, opB, Z, name="gelu")
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ---- the launcher's other ways: large tiles, split K, few columns, copies of unaligned operands ----
+
+def exact_product(pkg, L, kind, ta, tb, M, N, K, lay, kind_d=None, seed=1):
+    opA, opB, bias = rand_ints(M, K, seed), rand_ints(K, N, seed + 1), rand_ints(M, 1, seed + 2, -9, 9)[:, 0]
+    exact = opA @ opB + bias[:, None]
+    got, z = product(pkg, L, kind, ta, tb, opA, opB, bias=bias, name="relu", keep=True, lay=lay, kind_d=kind_d)
+    assert torch.equal(z, exact.to(TORCH[kind]).double())
+    assert torch.equal(got, exact.clamp(min=0).to(TORCH[kind_d or kind]).double())
+
+
+@pytest.mark.parametrize("kind,kind_d", [("bf16", None), ("f16", "f32")])
+@pytest.mark.parametrize("ta,tb", TRANS)
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 200), (4104, 4072, 648), (4100, 4099, 129), (2600, 8200, 321)])
+def test_large_products(pkg, L, kind, kind_d, ta, tb, M, N, K):
+    """Enough 256 x 256 tiles for every compute unit: whole and ragged, aligned and (pad 1) not."""
+    for lay in (Layout(), Layout(pad=8), Layout(pad=1, offset=1)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay, kind_d)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("ta,tb", TRANS)
+@pytest.mark.parametrize("M,N,K", [(256, 256, 4096), (128, 130, 8200), (257, 100, 5000), (1030, 70, 3001), (700, 300, 1001), (520, 1500, 2047)])
+def test_split_and_copied_products(pkg, L, kind, ta, tb, M, N, K):
+    """Few tiles and a long K; extents that are no multiple of 8, whose operands are copied."""
+    for lay in (Layout(), Layout(pad=8), Layout(pad=3, offset=5)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay)
+    opA, opB, Z = rand(M, K, 31, kind, K ** -0.5), rand(K, N, 32, kind), rand(M, N, 33, kind, 2.0)
+    d, ed, db, edb = gradient(opA, opB, Z, None, 1.0, 0.0, "gelu_tanh", kind)
+    got, gdb = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="gelu_tanh", lay=Layout(pad=1))
+    check(got, d, ed, "D")
+    check(gdb, db, edb, "dbias")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("M,K", [(5, 64), (100, 4096), (4100, 576), (5000, 64), (16400, 320), (33000, 128)])
+def test_few_columns(pkg, L, kind, N, M, K):
+    """Single tokens and small batches: fewer panels than waves, a panel count that does not divide, ragged last rows."""
+    exact_product(pkg, L, kind, "T", "N", M, N, K, Layout())
+    exact_product(pkg, L, kind, "T", "N", M, N, K, Layout(pad=8), kind_d="f32", seed=4)
+    opA, opB, Cm = rand_ints(M, K, 7), rand_ints(K, N, 8), rand_ints(M, N, 9, -9, 9)
+    got, _ = product(pkg, L, kind, "T", "N", opA, opB, alpha=2.0, beta=-1.0, Cm=Cm, in_place=True)
+    assert torch.equal(got, (2.0 * (opA @ opB) - Cm).to(TORCH[kind]).double())
+
+
+@pytest.mark.parametrize("kind", ["f32", "f64"])
+@pytest.mark.parametrize("ta,tb", TRANS)
+@pytest.mark.parametrize("M,N,K", [(256, 256, 4096), (1700, 1500, 1600), (700, 300, 1001)])
+def test_wide_products_split_and_cut(pkg, L, kind, ta, tb, M, N, K):
+    for lay in (Layout(), Layout(pad=1)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay)
+    opA, opB = rand_ints(M, K, 7), rand_ints(K, N, 8)
+    Cm, Z = rand_ints(M, N, 9, -9, 9), rand_ints(M, N, 10, -3, 3)
+    for in_place in (False, True):
+        got, _ = product(pkg, L, kind, ta, tb, opA, opB, alpha=3.0, beta=2.0, Cm=Cm, in_place=in_place)
+        assert torch.equal(got, 3.0 * (opA @ opB) + 2.0 * Cm)
+    got, db = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="relu")
+    want = (opA @ opB) * (Z > 0)
+    assert torch.equal(got, want) and torch.equal(db, want.sum(1))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("ta,tb,M,N,K", [("T", "N", 700, 300, 1001), ("N", "N", 256, 256, 4096), ("N", "T", 300, 200, 64), ("T", "T", 3, 5, 9)])
+def test_nothing_is_written_behind_the_workspace(pkg, L, kind, ta, tb, M, N, K):
+    opA, opB, Z = rand_ints(M, K, 1), rand_ints(K, N, 2), rand_ints(M, N, 3)
+    A, B = Mat(*((M, K) if ta == "N" else (K, M)), M if ta == "N" else K, kind).set(opA if ta == "N" else opA.T), Mat(*((K, N) if tb == "N" else (N, K)), K if tb == "N" else N, kind).set(opB if tb == "N" else opB.T)
+    Zb, D, db = Mat(M, N, M, kind).set(Z), Mat(M, N, M, kind, gap=7.0), Mat(M, 1, M, kind, gap=5.0)
+    need = L.pl_gemm_epilogue_workspace_bytes(TYPES[kind], ta.encode(), tb.encode(), M, N, K, 1)
+    ws = torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    pkg.check(L.pl_gemm_epilogue_grad(TYPES[kind], ta.encode(), tb.encode(), M, N, K, 1.0, A.ptr, A.ld, B.ptr, B.ld, ACTS["relu"], Zb.ptr, M, 0.0, None, 0, D.ptr, M, db.ptr,
+                                      ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream), "pl_gemm_epilogue_grad")
+    torch.cuda.synchronize()
+    assert bool((ws[need:] == 0xA5).all())
+    want = (opA @ opB) * (Z > 0)
+    assert torch.equal(D.get(), want.to(TORCH[kind]).double()) and torch.equal(db.get()[:, 0], want.sum(1).to(TORCH[kind]).double())
+
+
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_leading_dimensions_beyond_the_request_offsets(pkg, L, ta, tb):
+    """Columns 2^22 + 8 elements apart: what 32-bit offsets from a panel's start cannot span."""
+    M, N, K, ld = 20, 24, 20, (1 << 22) + 8
+    opA, opB = rand_ints(M, K, 1), rand_ints(K, N, 2)
+    A = Mat(*((M, K) if ta == "N" else (K, M)), ld, "bf16").set(opA if ta == "N" else opA.T)
+    B = Mat(*((K, N) if tb == "N" else (N, K)), ld, "bf16").set(opB if tb == "N" else opB.T)
+    D = Mat(M, N, ld, "bf16", gap=7.0)
+    ep = pkg.epilogue(type_d=3)
+    need = L.pl_gemm_epilogue_workspace_bytes(3, ta.encode(), tb.encode(), M, N, K, 0)
+    ws = workspace(need)
+    pkg.check(L.pl_gemm_epilogue(3, ta.encode(), tb.encode(), M, N, K, 1.0, A.ptr, ld, B.ptr, ld, C.byref(ep), 0.0, None, 0, D.ptr, ld, ws.data_ptr(), need,
+                                 torch.cuda.current_stream().cuda_stream), "pl_gemm_epilogue")
+    assert torch.equal(D.get(), (opA @ opB).to(torch.bfloat16).double()) and D.gaps_untouched()
+
+
+def test_a_result_beyond_4_gib(pkg, L):
+    """70000 x 40000 in 16 bits, 5.6 GB, with its gradient: rows and columns far behind 2^32 bytes."""
+    M, N, K = 70000, 40000, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w = torch.randint(-2, 3, (M, K), generator=g, device="cuda").to(torch.bfloat16)
+    x = torch.randint(-2, 3, (N, K), generator=g, device="cuda").to(torch.bfloat16)
+    y = torch.full((N, M), 9.0, dtype=torch.bfloat16, device="cuda")
+    ep = pkg.epilogue(type_d=3, activation=ACTS["relu"])
+    s = torch.cuda.current_stream().cuda_stream
+    need = L.pl_gemm_epilogue_workspace_bytes(3, b"T", b"N", M, N, K, 0)
+    ws = workspace(need)
+    pkg.check(L.pl_gemm_epilogue(3, b"T", b"N", M, N, K, 1.0, w.data_ptr(), K, x.data_ptr(), K, C.byref(ep), 0.0, None, 0, y.data_ptr(), M, ws.data_ptr(), need, s), "pl_gemm_epilogue")
+    rows = torch.tensor([0, 1, 255, 256, 20000, 30679, 30680, 39999], device="cuda")
+    assert torch.equal(y[rows].float(), (x[rows].float() @ w.float().T).clamp(min=0))
+    db = torch.zeros(M, dtype=torch.bfloat16, device="cuda")
+    need = L.pl_bias_act_grad_workspace_bytes(3, M, N)
+    ws = workspace(need)
+    before = y[rows].clone()
+    pkg.check(L.pl_bias_act_grad(3, ACTS["relu"], M, N, y.data_ptr(), M, y.data_ptr(), M, y.data_ptr(), M, db.data_ptr(), ws.data_ptr(), need, s), "pl_bias_act_grad")
+    assert torch.equal(y[rows], before)
+    # whole numbers: columns summed in 32 bits are exact (below 2^24)
+    some = torch.tensor([0, 1, 35000, M - 1], device="cuda")
+    assert torch.equal(db[some].float(), y[:, some].float().sum(0).to(torch.bfloat16).float())
+
+
+# ---- as they are used together ----
+
+class Layer2:
+    """Two linear layers with an activation between them, row-major as a program holds them: the calls of a training step."""
+
+    def __init__(self, pkg, L, kind, tokens, width, hidden, name, seed):
+        self.pkg, self.L, self.kind, self.t, self.w, self.h, self.name = pkg, L, kind, tokens, width, hidden, name
+        self.code, self.act = TYPES[kind], ACTS[name]
+        g = torch.Generator().manual_seed(seed)
+        new = lambda *shape, scale=1.0: (torch.randn(*shape, generator=g, dtype=torch.float64) * scale).to(TORCH[kind]).cuda()  # noqa: E731
+        self.x, self.r, self.dy = new(tokens, width), new(tokens, width), new(tokens, width, scale=0.1)
+        self.w1, self.b1 = new(hidden, width, scale=width ** -0.5), new(hidden, scale=0.3)
+        self.w2, self.b2 = new(width, hidden, scale=hidden ** -0.5), new(width, scale=0.3)
+        z = lambda *shape, t=kind: torch.zeros(*shape, dtype=TORCH[t], device="cuda")  # noqa: E731
+        wide = "f64" if kind == "f64" else "f32"
+        self.wide = wide
+        self.z1, self.a1, self.y = z(tokens, hidden), z(tokens, hidden), z(tokens, width)
+        self.dz1, self.dx = z(tokens, hidden), z(tokens, width)
+        self.gb1, self.gb2 = z(hidden), z(width)
+        self.gw1, self.gw2 = z(hidden, width, t=wide), z(width, hidden, t=wide)
+        self.norm = torch.zeros(1, dtype=torch.float64, device="cuda")
+        q = lambda ta, tb, m, n, k, d: L.pl_gemm_epilogue_workspace_bytes(self.code, ta, tb, m, n, k, d)  # noqa: E731
+        need = max(q(b"T", b"N", hidden, tokens, width, 0), q(b"T", b"N", width, tokens, hidden, 0), q(b"N", b"N", hidden, tokens, width, 1), q(b"N", b"N", width, tokens, hidden, 0),
+                   q(b"N", b"T", hidden, width, tokens, 0), q(b"N", b"T", width, hidden, tokens, 0), L.pl_bias_act_grad_workspace_bytes(self.code, width, tokens), L.pl_grad_norm_workspace_bytes(4))
+        self.need, self.ws = need, workspace(need)
+        grads = [self.gw1, self.gb1, self.gw2, self.gb2]
+        self.n = len(grads)
+        self.ptrs, self.counts = (C.c_void_p * 4)(*[t.data_ptr() for t in grads]), (C.c_longlong * 4)(*[t.numel() for t in grads])
+        self.types = (C.c_int * 4)(TYPES[wide], self.code, TYPES[wide], self.code)
+
+    def gemm(self, s, ta, tb, m, n, k, a, b, d, ep, beta=0.0, c=None):
+        ld = lambda t: t.stride(0)  # noqa: E731
+        self.pkg.check(self.L.pl_gemm_epilogue(self.code, ta, tb, m, n, k, 1.0, a.data_ptr(), ld(a), b.data_ptr(), ld(b), C.byref(ep), beta, c.data_ptr() if c is not None else None,
+                                               ld(c) if c is not None else 0, d.data_ptr(), ld(d), self.ws.data_ptr(), self.need, s), "pl_gemm_epilogue")
+
+    def step(self, s, limit):
+        pkg, L, t, w, h = self.pkg, self.L, self.t, self.w, self.h
+        ep = pkg.epilogue
+        up = ep(bias=self.b1.data_ptr(), activation=self.act, type_d=self.code, preact=self.z1.data_ptr(), ld_preact=h)
+        self.gemm(s, b"T", b"N", h, t, w, self.w1, self.x, self.a1, up)
+        self.gemm(s, b"T", b"N", w, t, h, self.w2, self.a1, self.y, ep(bias=self.b2.data_ptr(), type_d=self.code), beta=1.0, c=self.r)
+        pkg.check(L.pl_bias_act_grad(self.code, 0, w, t, self.dy.data_ptr(), w, None, 0, None, 0, self.gb2.data_ptr(), self.ws.data_ptr(), self.need, s), "db2")
+        pkg.check(L.pl_gemm_epilogue_grad(self.code, b"N", b"N", h, t, w, 1.0, self.w2.data_ptr(), h, self.dy.data_ptr(), w, self.act, self.z1.data_ptr(), h, 0.0, None, 0,
+                                          self.dz1.data_ptr(), h, self.gb1.data_ptr(), self.ws.data_ptr(), self.need, s), "dz1")
+        wide = ep(type_d=TYPES[self.wide])
+        self.gemm(s, b"N", b"T", h, w, t, self.a1, self.dy, self.gw2, wide, beta=1.0, c=self.gw2)
+        self.gemm(s, b"N", b"T", w, h, t, self.x, self.dz1, self.gw1, wide, beta=1.0, c=self.gw1)
+        self.gemm(s, b"N", b"N", w, t, h, self.w1, self.dz1, self.dx, ep(type_d=self.code))
+        pkg.check(L.pl_grad_norm_clip(self.n, self.ptrs, self.counts, self.types, self.ptrs, limit, 1e-6, self.norm.data_ptr(), self.ws.data_ptr(), self.need, s), "clip")
+
+    def outputs(self):
+        return [t.clone() for t in (self.y, self.z1, self.a1, self.dz1, self.dx, self.gw1, self.gw2, self.gb1, self.gb2, self.norm)]
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+def test_a_training_step_against_differences(pkg, L, name):
+    """fp64, 5 tokens: every gradient of loss = sum(dy * y) against central differences of the library's own forward pass.
+    With a step of 1e-6 the differences are off by about 1e-12 (third derivatives) + 1e-16 * |loss| / 1e-6."""
+    m = Layer2(pkg, L, "f64", 5, 6, 9, name, 3)
+    m.step(stream(), 1e30)
+    torch.cuda.synchronize()
+    grads = {"w1": m.gw1.clone(), "b1": m.gb1.clone(), "w2": m.gw2.clone(), "b2": m.gb2.clone(), "x": m.dx.clone()}
+    assert abs(float(m.norm) - math.sqrt(sum(float((grads[k] ** 2).sum()) for k in ("w1", "b1", "w2", "b2")))) < 1e-12
+    for k, g in grads.items():
+        p = getattr(m, k)
+        flat, want = p.view(-1), []
+        for i in range(flat.numel()):
+            old = float(flat[i])
+            loss = []
+            for e in (1e-6, -1e-6):
+                flat[i] = old + e
+                up = pkg.epilogue(bias=m.b1.data_ptr(), activation=m.act, type_d=0)
+                m.gemm(stream(), b"T", b"N", m.h, m.t, m.w, m.w1, m.x, m.a1, up)
+                m.gemm(stream(), b"T", b"N", m.w, m.t, m.h, m.w2, m.a1, m.y, pkg.epilogue(bias=m.b2.data_ptr(), type_d=0), beta=1.0, c=m.r)
+                loss.append(float((m.y * m.dy).sum()))
+            flat[i] = old
+            want.append((loss[0] - loss[1]) / 2e-6)
+        want = torch.tensor(want, dtype=torch.float64, device="cuda").view(g.shape)
+        assert float((g - want).abs().max()) < 1e-8, k
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("tokens,width,hidden", [(64, 128, 256), (333, 136, 1000), (37, 130, 259)])
+def test_a_training_step_against_64_bits(pkg, L, kind, tokens, width, hidden):
+    """A whole step, each call held to its definition on what the call before it really left."""
+    m = Layer2(pkg, L, kind, tokens, width, hidden, "gelu_tanh", 5)
+    m.step(stream(), 1e30)
+    torch.cuda.synchronize()
+    T = lambda t: t.double().T  # noqa: E731
+    x, w1, w2, dy = (t.double() for t in (m.x, m.w1, m.w2, m.dy))
+    z, ez, a, ea = forward(w1, x.T, m.b1.double(), None, 1.0, 0.0, "gelu_tanh", kind, kind)
+    check(T(m.z1), z, ez, "z1")
+    check(T(m.a1), a, ea, "a1")
+    _, _, y, ey = forward(w2, T(m.a1), m.b2.double(), m.r.double().T, 1.0, 1.0, "none", kind, kind)
+    check(T(m.y), y, ey, "y")
+    d, ed, db, edb = gradient(w2.T, dy.T, T(m.z1), None, 1.0, 0.0, "gelu_tanh", kind)
+    check(T(m.dz1), d, ed, "dz1")
+    check(m.gb1.double(), db, edb, "gb1")
+    wide = "f32"
+    _, _, g, eg = forward(m.a1.double().T, dy, None, None, 1.0, 0.0, "none", kind, wide)
+    check(T(m.gw2), g, eg, "gw2")
+    _, _, g, eg = forward(x.T, m.dz1.double(), None, None, 1.0, 0.0, "none", kind, wide)
+    check(T(m.gw1), g, eg, "gw1")
+    _, _, g, eg = forward(w1.T, T(m.dz1), None, None, 1.0, 0.0, "none", kind, kind)
+    check(T(m.dx), g, eg, "dx")
+
+
+@pytest.mark.parametrize("kind,tokens,width,hidden", [("bf16", 96, 256, 512), ("f16", 41, 130, 515), ("f32", 64, 96, 200), ("bf16", 1, 4096, 512)])
+def test_a_captured_step_replays(pkg, L, kind, tokens, width, hidden):
+    """The step recorded into a graph, replayed on new inputs with eager work and synchronisations in between, against the
+    eager step on the same inputs, bit for bit."""
+    eager, captured = (Layer2(pkg, L, kind, tokens, width, hidden, "silu", 7) for _ in range(2))
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    captured.step(stream(), 0.5)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        captured.step(torch.cuda.current_stream().cuda_stream, 0.5)
+    g = torch.Generator().manual_seed(1)
+    for m in (eager, captured):
+        for t in (m.gw1, m.gw2, m.gb1, m.gb2):
+            t.zero_()
+    for replay in range(4):
+        x = torch.randn(tokens, width, generator=g).to(TORCH[kind]).cuda()
+        eager.x.copy_(x), captured.x.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.step(stream(), 0.5)
+        torch.cuda.synchronize()
+        for a, b in zip(eager.outputs(), captured.outputs()):
+            assert torch.equal(a, b), replay
+
+
+def test_two_streams_and_two_threads_at_once(pkg, L):
+    """Steps with workspaces of their own on two streams, issued by two host threads, leave what they leave alone."""
+    import threading
+    alone = Layer2(pkg, L, "bf16", 200, 512, 1030, "gelu", 9)
+    alone.step(stream(), 0.5)
+    torch.cuda.synchronize()
+    want = alone.outputs()
+    models = [Layer2(pkg, L, "bf16", 200, 512, 1030, "gelu", 9) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(m, s):
+        try:
+            for _ in range(10):
+                with torch.cuda.stream(s):
+                    for t in (m.gw1, m.gw2):
+                        t.zero_()
+                m.step(s.cuda_stream, 0.5)
+        except Exception as e:   # reported by the main thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=a) for a in zip(models, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for m in models:
+        for a, b in zip(want, m.outputs()):
+            assert torch.equal(a, b)
+
