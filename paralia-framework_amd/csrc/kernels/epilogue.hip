@@ -168,7 +168,7 @@ int launch_act_grad(int type, int act, long M, long N, const void* dY, long lddy
 }  // namespace plk
 
 extern "C" long pl_bias_act_grad_workspace_bytes(int type, long M, long N) {
-  if (!plk::valid_type(type) || M <= 0 || N <= 0 || M > INT32_MAX || N > INT32_MAX) return 0;
+  if (!plk::valid_type(type) || M <= 0 || N <= 0 || M > (1L << 27) || N > INT32_MAX) return 0;
   return plk::epilogue_pass_rows(type, M, N) * M * (type == PL_TYPE_F64 ? 8 : 4);
 }
 
@@ -178,7 +178,7 @@ extern "C" int pl_bias_act_grad(int type, int activation, long M, long N, const 
   const char* const who = "pl_bias_act_grad";
   if (!valid_type(type)) return refuse(PL_ERR_ARG, who, "unknown element type");
   if (!valid_act(activation)) return refuse(PL_ERR_ARG, who, "unknown activation");
-  if (M < 0 || N < 0 || M > INT32_MAX || N > INT32_MAX) return refuse(PL_ERR_DIM, who, "dimension out of range");
+  if (M < 0 || N < 0 || M > (1L << 27) || N > INT32_MAX) return refuse(PL_ERR_DIM, who, "dimension out of range");
   const bool need_z = activation != PL_ACT_NONE;
   if (lddy < (M > 1 ? M : 1) || (need_z && ldz < (M > 1 ? M : 1)) || (dZ && lddz < (M > 1 ? M : 1))) return refuse(PL_ERR_LD, who, "leading dimension below M");
   if (M == 0) return PL_OK;
@@ -196,6 +196,11 @@ extern "C" int pl_bias_act_grad(int type, int activation, long M, long N, const 
   if (dZ) {
     if (!same_or_apart(dz, Range{dY, lddy, M, N, es}) || (need_z && !same_or_apart(dz, Range{Z, ldz, M, N, es}))) return refuse(PL_ERR_ARG, who, "dZ overlaps an operand it is not");
     if (dbias && overlap(dz, Range{dbias, M, M, 1, es})) return refuse(PL_ERR_ARG, who, "dZ overlaps dbias");
+  }
+  if (dbias) {
+    const Range dy = {dY, lddy, M, N, es}, z = {need_z ? Z : nullptr, ldz, M, N, es}, db = {dbias, M, M, 1, es}, work = bytes_at(workspace, pl_bias_act_grad_workspace_bytes(type, M, N));
+    if (overlap(db, dy) || overlap(db, z)) return refuse(PL_ERR_ARG, who, "dbias overlaps an operand");
+    if (overlap(work, dy) || overlap(work, z) || overlap(work, dz) || overlap(work, db)) return refuse(PL_ERR_ARG, who, "the workspace overlaps an operand");
   }
   switch (type) {
     case PL_TYPE_F64: return launch_act_grad<double>(type, activation, M, N, dY, lddy, Z, ldz, dZ, lddz, dbias, workspace, s);

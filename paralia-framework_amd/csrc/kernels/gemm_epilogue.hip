@@ -72,6 +72,7 @@ int run_product(Call& c) {
   const long M = c.M, N = c.N, K = c.K;
   if (M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX || ((M + 127) / 128) * ((N + 127) / 128) >= (1L << 24))
     return refuse(PL_ERR_DIM, who, "dimension out of range");
+  if (c.dbias && M > (1L << 27)) return refuse(PL_ERR_DIM, who, "more than 2^27 rows with a bias gradient");
   auto short_ld = [](long ld, long rows) { return ld < (rows > 1 ? rows : 1); };
   Epilogue& ep = c.ep;
   const bool uses_c = ep.beta != 0.0, uses_z = c.grad && ep.act != PL_ACT_NONE;
@@ -96,6 +97,9 @@ int run_product(Call& c) {
   if (!same_or_apart(d, rc) || !same_or_apart(d, z)) return refuse(PL_ERR_ARG, who, "D overlaps C or Z without being it");
   const Workspace w = workspace_for(c.type, at, bt, M, N, K, c.dbias != nullptr);
   if (w.bytes() > 0 && (!c.workspace || !aligned_to(c.workspace, 16) || c.workspace_bytes < w.bytes())) return refuse(PL_ERR_ARG, who, "workspace null, too small or not 16-byte aligned");
+  const Range work = bytes_at(w.bytes() > 0 ? c.workspace : nullptr, w.bytes());
+  for (const Range& r : {a, b, d, p, rc, z, bias, db})
+    if (overlap(work, r)) return refuse(PL_ERR_ARG, who, "the workspace overlaps an operand");
   char* const ws = (char*)c.workspace;
   ep.alpha = empty ? 0.0 : c.alpha;
   ep.partial = c.dbias ? ws + w.product : nullptr;

@@ -168,7 +168,8 @@ inline Span span_of(const void* p, long long count, int type) {
 
 // Refuses what the kernels cannot take: they would scale a tensor that is listed twice twice, or read one tensor's
 // gradients after writing another's.
-int check_list(const char* who, long n, const void* const* src, const long long* counts, const int* types, void* const* dst) {
+int check_list(const char* who, long n, const void* const* src, const long long* counts, const int* types, void* const* dst, const double* norm, const void* workspace,
+               long workspace_bytes) {
   if (n < 0 || n > (1L << 20)) return refuse(PL_ERR_DIM, who, "tensor count out of range");
   if (n == 0) return PL_OK;
   if (!src || !counts || !types) return refuse(PL_ERR_NULL, who, "null list");
@@ -178,6 +179,11 @@ int check_list(const char* who, long n, const void* const* src, const long long*
     if (counts[i] == 0) continue;
     if (!src[i] || (dst && !dst[i])) return refuse(PL_ERR_NULL, who, "null tensor");
     if (!aligned_to(src[i], type_size(types[i])) || (dst && !aligned_to(dst[i], type_size(types[i])))) return refuse(PL_ERR_ARG, who, "tensor not aligned to its element size");
+    for (const void* p : {src[i], dst ? (const void*)dst[i] : nullptr}) {
+      if (!p) continue;
+      const Range t = bytes_at(p, (long)counts[i] * type_size(types[i]));
+      if (overlap(t, bytes_at(norm, 8)) || overlap(t, bytes_at(workspace, workspace_bytes))) return refuse(PL_ERR_ARG, who, "norm or workspace overlaps a tensor");
+    }
   }
   if (!dst) return PL_OK;
   std::vector<Span> out, in;
@@ -291,7 +297,7 @@ extern "C" int pl_grad_norm(long n, const void* const* grads, const long long* c
   using namespace plk;
   const char* const who = "pl_grad_norm";
   return without_exceptions(who, [&]() -> int {
-    int rc = check_list(who, n, grads, counts, types, nullptr);
+    int rc = check_list(who, n, grads, counts, types, nullptr, norm, workspace, pl_grad_norm_workspace_bytes(n));
     if (rc == PL_OK) rc = check_norm_args(who, n, norm, workspace, workspace_bytes);
     return rc != PL_OK ? rc : grad_norm_only(n, grads, counts, types, norm, (double*)workspace, (hipStream_t)stream);
   });
@@ -303,7 +309,7 @@ extern "C" int pl_grad_clip(long n, const void* const* grads, const long long* c
   const char* const who = "pl_grad_clip";
   return without_exceptions(who, [&]() -> int {
     if (n > 0 && !outs) return refuse(PL_ERR_NULL, who, "null list");
-    const int rc = check_list(who, n, grads, counts, types, outs);
+    const int rc = check_list(who, n, grads, counts, types, outs, norm, nullptr, 0);
     if (rc != PL_OK) return rc;
     if (!norm) return refuse(PL_ERR_NULL, who, "null norm");
     if (!aligned_to(norm, 8) || !valid_limit(max_norm, eps)) return refuse(PL_ERR_ARG, who, "max_norm or eps negative or NaN, or norm not 8-byte aligned");
@@ -317,7 +323,7 @@ extern "C" int pl_grad_norm_clip(long n, const void* const* grads, const long lo
   const char* const who = "pl_grad_norm_clip";
   return without_exceptions(who, [&]() -> int {
     if (n > 0 && !outs) return refuse(PL_ERR_NULL, who, "null list");
-    int rc = check_list(who, n, grads, counts, types, outs);
+    int rc = check_list(who, n, grads, counts, types, outs, norm, workspace, pl_grad_norm_workspace_bytes(n));
     if (rc == PL_OK) rc = check_norm_args(who, n, norm, workspace, workspace_bytes);
     if (rc != PL_OK) return rc;
     if (!valid_limit(max_norm, eps)) return refuse(PL_ERR_ARG, who, "max_norm or eps negative or NaN");

@@ -43,6 +43,7 @@ inline bool overlap(const Range& a, const Range& b) {
   }
   return true;
 }
+inline Range bytes_at(const void* p, long bytes) { return Range{p, bytes, bytes, 1, 1}; }
 // the same matrix, element for element, or no byte in common
 inline bool same_or_apart(const Range& a, const Range& b) {
   return (a.p == b.p && (a.ld == b.ld || a.cols == 1) && a.size == b.size) || !overlap(a, b);
@@ -120,13 +121,13 @@ inline bool can_request(const void* A, long lda, const void* B, long ldb) {
 // Operands that cannot be requested are multiplied from aligned copies where that pays: a panel of unaligned 16-byte loads
 // takes a compute unit 0.7 - 1.1 us longer than a requested one (misaligned lanes are served one by one), each operand's
 // panels are loaded by every tile in its row or column, and the copies cost one launch and one pass over the operands
-// (4100 x 1023 x 2052, rows of an odd number of elements: 70 -> @ us).  The space is set aside by the shape alone: where a
+// (4100 x 1023 x 2052, rows of an odd number of elements: 70 -> 47 us).  The space is set aside by the shape alone: where a
 // contiguous extent is no multiple of 8, so that dense operands could not be aligned.
 struct HalfCopies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
 inline HalfCopies half_copies(bool at, bool bt, long M, long N, long K) {
   const long ext_a = at ? K : M, rows_a = at ? M : K, ext_b = bt ? N : K, rows_b = bt ? K : N;
   HalfCopies c = {0, 0, 0, 0};
-  if ((ext_a % 8 == 0 && ext_b % 8 == 0) || ext_a < 8 || ext_b < 8) return c;
+  if ((ext_a % 8 == 0 && ext_b % 8 == 0) || ext_a < 8 || ext_b < 8 || K > (1L << 30)) return c;
   const double tiles = (double)((M + 127) / 128) * (double)((N + 127) / 128);
   const double slow_us = 0.8 * (double)(K / H_BK) * (tiles > 256.0 ? tiles / 256.0 : 1.0), copy_us = 6.0 + 4.0 * (double)K * (double)(M + N) / 3e6;
   if (slow_us < copy_us) return c;

@@ -112,6 +112,24 @@ def test_gradient_clipping_refuses(L):
     assert L.pl_grad_norm_workspace_bytes(0) == 0 and L.pl_grad_norm_workspace_bytes(1) >= 8192
 
 
+def test_workspaces_that_overlap_operands_are_refused(pkg, L):
+    need = L.pl_gemm_epilogue_workspace_bytes(3, b"N", b"N", 64, 32, 16, 1)
+    for at in (A, B + 128, D - need + 16, Z, DB - 16):
+        assert grad(L, ws=at & ~15, wsb=1 << 20) == 7, hex(at)
+        assert b"workspace" in L.pl_last_error()
+    for at in (A, Z, D, DB):
+        assert act_grad(L, ws=at, wsb=1 << 20) == 7
+    assert act_grad(L, db=A + 64) == 7 and act_grad(L, db=Z) == 7
+    for over in (dict(norm=A + 8), dict(norm=B + 392), dict(ws=A), dict(ws=A - 4096)):
+        assert clip(L, [A, B], [100, 200], [1, 3], [A, B], **over) == 7
+        assert b"overlaps a tensor" in L.pl_last_error()
+
+
+def test_rows_beyond_the_fold(L):
+    assert act_grad(L, M=(1 << 27) + 1, N=1, lddy=1 << 28, ldz=1 << 28, lddz=1 << 28) == 2
+    assert grad(L, M=(1 << 27) + 1, N=1, K=1, lda=1 << 28, ldz=1 << 28, ldd=1 << 28) == 2
+
+
 def test_nothing_to_do_is_no_error(pkg, L):
     assert call(L, pkg, M=0, lda=16, ldd=1) == 0
     assert call(L, pkg, N=0) == 0
