@@ -246,7 +246,10 @@ typedef struct pl_epilogue {
  * and B.  D may be C itself (same pointer and leading dimension), otherwise no output may overlap another operand.
  * With beta = 1, no activation and C = D this accumulates a weight gradient (16-bit operands: into fp32, if type_D says
  * so).  workspace: pl_gemm_epilogue_workspace_bytes(type, transA, transB, M, N, K, 0) bytes, 16-byte aligned (null where
- * that is 0); it must not be shared by calls that may overlap, and a captured graph keeps using the one it was given. */
+ * that is 0); it must not be shared by calls that may overlap, and a captured graph keeps using the one it was given.
+ * 16-bit operands whose pointers and leading dimensions are multiples of 16 bytes are requested straight into LDS; others
+ * take about twice as long, or are copied into the workspace first where a contiguous extent is no multiple of 8 elements
+ * (the only case whose space is set aside) and the product is long enough. */
 long pl_gemm_epilogue_workspace_bytes(int type, char transA, char transB, long M, long N, long K, int with_dbias);
 int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda, const void* B,
                      long ldb, const pl_epilogue* epilogue, double beta, const void* C, long ldc, void* D, long ldd, void* workspace,
@@ -277,7 +280,7 @@ int pl_grad_norm(long n, const void* const* grads, const long long* counts, cons
                  long workspace_bytes, void* stream);
 /* outs[i] <- grads[i] * min(1, max_norm / (*norm + eps)) with a norm that is on the device already (of several GPUs'
  * gradients, say).  outs[i] may be grads[i] itself; any other overlap of an output with a tensor of the list is refused,
- * the same tensor listed twice among them.  max_norm and eps must not be negative.  A NaN norm makes every element NaN. */
+ * the same tensor listed twice among them, and so is one with norm or the workspace.  max_norm and eps must not be negative.  A NaN norm makes every element NaN. */
 int pl_grad_clip(long n, const void* const* grads, const long long* counts, const int* types, void* const* outs, double max_norm,
                  double eps, const double* norm, void* stream);
 /* both in one call, one launch fewer */
