@@ -103,16 +103,13 @@ int launch_epilogue_pass(long M, long N, const TP* P, long ldP, long slice, int 
   const long ranges = pass_ranges<T>(M, N), per = (N + ranges - 1) / ranges;
   const dim3 grid((unsigned)((M + 64 * VEC - 1) / (64 * VEC)), (unsigned)((N + per - 1) / per));
 #define LAUNCH(SLICES) \
-  hipLaunchKernelGGL((epilogue_pass_kernel<TP, T, TD, GRAD, SLICES, VEC>), grid, dim3(PASS_THREADS), 0, stream, M, N, per, P, ldP, slice, slices, ep)
+  return launch(epilogue_pass_kernel<TP, T, TD, GRAD, SLICES, VEC>, grid, dim3(PASS_THREADS), stream, M, N, per, P, ldP, slice, slices, ep)
   // (a 16-bit operand is no slice of a product; the fp64 gradient has no scalar registers left for slices)
   if constexpr (sizeof(TP) == sizeof(wide_t<T>) && !(GRAD && sizeof(T) == 8)) {
     if (slices > 1) LAUNCH(true);
-    else LAUNCH(false);
-  } else {
-    LAUNCH(false);
   }
+  LAUNCH(false);
 #undef LAUNCH
-  return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
 }
 
 template <typename T> long pass_partial_rows(long M, long N) {
@@ -121,8 +118,7 @@ template <typename T> long pass_partial_rows(long M, long N) {
 }
 
 template <typename T> int launch_bias_fold(long M, long rows, const void* partial, void* dbias, hipStream_t stream) {
-  hipLaunchKernelGGL(bias_fold_kernel<T>, dim3((unsigned)((M + 15) / 16)), dim3(256), 0, stream, M, rows, (const wide_t<T>*)partial, (T*)dbias);
-  return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
+  return launch(bias_fold_kernel<T>, dim3((unsigned)((M + 15) / 16)), dim3(256), stream, M, rows, (const wide_t<T>*)partial, (T*)dbias);
 }
 
 int bias_fold(int type, long M, long rows, const void* partial, void* dbias, hipStream_t stream) {

@@ -11,14 +11,18 @@ namespace plk {
 // The workspace of one call, in the order it is laid out: the product or its slices, the partial bias gradients, aligned copies of 16-bit operands.
 struct Workspace { long product, partial, copies; long bytes() const { return product + partial + copies; } };
 inline long round16(long b) { return (b + 15) & ~15L; }
-inline Workspace workspace_for(int type, bool at, bool bt, long M, long N, long K, bool dbias) {
+inline Workspace workspace_for(int type, const HalfPlan& p, const HalfCopies& copies, bool at, bool bt, long M, long N, long K, bool dbias) {
   Workspace w = {0, 0, 0};
   const long wide = type == PL_TYPE_F64 ? 8 : 4;
   if (type_size(type) == 2) {
-    const HalfPlan p = plan_half(at, bt, M, N, K);
     if (p.splits > 1 || p.tile == 0) w.product = round16((long)p.splits * M * N * 4);
-    if (dbias) w.partial = round16(half_partial_rows({p.tile == 256 ? 128 : p.tile, p.splits, 0}, type, M, N) * M * wide);   // (unaligned operands: the small tile)
-    w.copies = half_copies(at, bt, M, N, K).bytes();
+    if (dbias) {
+      // the small tile's, which unaligned operands are given to, or the pass's: the larger, because a product that turns
+      // out to be empty (alpha = 0) is not split
+      const long tile_rows = half_partial_rows({128, 1, 0}, type, M, N), pass_rows = half_partial_rows({0, 1, 0}, type, M, N);
+      w.partial = round16((tile_rows > pass_rows ? tile_rows : pass_rows) * M * wide);
+    }
+    w.copies = copies.bytes();
   } else {
     // the slices of a product alone on the device, or the product and behind it the slices of its tail
     w.product = round16(M * N * wide) + round16(pl_gemm_tile_alone_workspace_bytes(at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, type_size(type)));
@@ -54,8 +58,7 @@ int half_copy(const void* A, long lda, void* copy_a, const void* B, long ldb, vo
   const HalfCopyJob b = {(const short*)B, (short*)copy_b, ldb, to.ld_b, bt ? c.K : c.N, to.bytes_b / (2 * to.ld_b), (int)(bt ? c.N : c.K)};
   const long most = (to.bytes_a > to.bytes_b ? to.bytes_a : to.bytes_b) / 16;
   const long blocks = (most + 255) / 256;
-  hipLaunchKernelGGL(half_copy_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), 0, c.stream, a, b);
-  return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
+  return launch(half_copy_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), c.stream, a, b);
 }
 
 bool plain_product(const Call& c) {
@@ -95,7 +98,14 @@ int run_product(Call& c) {
     return refuse(PL_ERR_ARG, who, "an output overlaps another operand");
   // D may be C, or Z, itself: an element is read before it is written, by the same thread
   if (!same_or_apart(d, rc) || !same_or_apart(d, z)) return refuse(PL_ERR_ARG, who, "D overlaps C or Z without being it");
-  const Workspace w = workspace_for(c.type, at, bt, M, N, K, c.dbias != nullptr);
+  const bool few = es == 2 && !empty && few_columns(c, at, bt);   // (a kernel that needs no workspace, and no plan)
+  HalfPlan plan = {0, 1, 0};
+  HalfCopies copies = {0, 0, 0, 0};
+  Workspace w = {0, 0, 0};
+  if (!few) {
+    if (es == 2) plan = plan_half(at, bt, M, N, K), copies = half_copies(at, bt, M, N, K);
+    w = workspace_for(c.type, plan, copies, at, bt, M, N, K, c.dbias != nullptr);
+  }
   if (w.bytes() > 0 && (!c.workspace || !aligned_to(c.workspace, 16) || c.workspace_bytes < w.bytes())) return refuse(PL_ERR_ARG, who, "workspace null, too small or not 16-byte aligned");
   const Range work = bytes_at(w.bytes() > 0 ? c.workspace : nullptr, w.bytes());
   for (const Range& r : {a, b, d, p, rc, z, bias, db})
@@ -107,9 +117,7 @@ int run_product(Call& c) {
   int rc_;
   long rows;
   if (es == 2) {
-    HalfPlan plan = plan_half(at, bt, M, N, K);
     if (empty) plan.splits = 1, plan.kchunk = 0;
-    const HalfCopies copies = half_copies(at, bt, M, N, K);
     if (!empty && copies.bytes() > 0 && !can_request(c.A, c.lda, c.B, c.ldb) && in_offset_range(copies.ld_a, copies.ld_b)) {
       char* const copy_a = ws + w.product + w.partial;
       rc_ = half_copy(c.A, c.lda, copy_a, c.B, c.ldb, copy_a + copies.bytes_a, c, at, bt, copies);
@@ -120,8 +128,8 @@ int run_product(Call& c) {
       c.padded = true;
     }
     if (plan.tile == 256 && !can_request(c.A, c.lda, c.B, c.ldb)) plan.tile = 128;
-    rows = half_partial_rows(plan, c.type, M, N);
-    const bool f16 = c.type == PL_TYPE_F16, sliced = (plan.tile == 0 || plan.splits > 1) && !few_columns(c, at, bt);
+    rows = few ? 0 : half_partial_rows(plan, c.type, M, N);
+    const bool f16 = c.type == PL_TYPE_F16, sliced = !few && (plan.tile == 0 || plan.splits > 1);
     if (sliced) {
       rc_ = f16 ? half_slices_f16(c, plan, at, bt, ws) : half_slices_bf16(c, plan, at, bt, ws);
       if (rc_ == PL_OK) rc_ = epilogue_pass(c.type, c.type_d, c.grad, M, N, ws, M, M * N, plan.splits, ep, c.stream);
@@ -154,7 +162,8 @@ extern "C" long pl_gemm_epilogue_workspace_bytes(int type, char transA, char tra
   using namespace plk;
   if (!valid_type(type) || M <= 0 || N <= 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
   const bool at = transA == 'T' || transA == 't', bt = transB == 'T' || transB == 't';
-  return workspace_for(type, at, bt, M, N, K, with_dbias != 0).bytes();
+  const bool half = type_size(type) == 2;
+  return workspace_for(type, half ? plan_half(at, bt, M, N, K) : HalfPlan{0, 1, 0}, half ? half_copies(at, bt, M, N, K) : HalfCopies{0, 0, 0, 0}, at, bt, M, N, K, with_dbias != 0).bytes();
 }
 
 extern "C" int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda, const void* B, long ldb,

@@ -186,21 +186,27 @@ int check_list(const char* who, long n, const void* const* src, const long long*
     }
   }
   if (!dst) return PL_OK;
-  std::vector<Span> out, in;
-  out.reserve(n);
+  // (lists of up to 256 tensors on the stack: two allocations are a microsecond of a small call)
+  Span few_out[256], few_in[256];
+  std::vector<Span> many;
+  Span* out = few_out;
+  Span* in = few_in;
+  if (n > 256) many.resize(2 * n), out = many.data(), in = out + n;
+  long outs = 0, ins = 0;
   for (long i = 0; i < n; ++i) {
     if (counts[i] == 0) continue;
-    out.push_back(span_of(dst[i], counts[i], types[i]));
-    if (src[i] != dst[i]) in.push_back(span_of(src[i], counts[i], types[i]));
+    out[outs++] = span_of(dst[i], counts[i], types[i]);
+    if (src[i] != dst[i]) in[ins++] = span_of(src[i], counts[i], types[i]);
   }
   auto by_first = [](const Span& a, const Span& b) { return a.first < b.first; };
-  if (!std::is_sorted(out.begin(), out.end(), by_first)) std::sort(out.begin(), out.end(), by_first);
-  for (size_t i = 1; i < out.size(); ++i)
+  if (!std::is_sorted(out, out + outs, by_first)) std::sort(out, out + outs, by_first);
+  for (long i = 1; i < outs; ++i)
     if (out[i].first < out[i - 1].last) return refuse(PL_ERR_ARG, who, "two tensors of the list are written to the same memory");
   // outputs are disjoint and in order: an input that is not its own output must lie between two of them
-  for (const Span& s : in) {
-    auto it = std::upper_bound(out.begin(), out.end(), s, by_first);
-    if ((it != out.end() && it->first < s.last) || (it != out.begin() && (it - 1)->last > s.first)) return refuse(PL_ERR_ARG, who, "a tensor is written over another one of the list");
+  for (long i = 0; i < ins; ++i) {
+    const Span& s = in[i];
+    const Span* const it = std::upper_bound(out, out + outs, s, by_first);
+    if ((it != out + outs && it->first < s.last) || (it != out && (it - 1)->last > s.first)) return refuse(PL_ERR_ARG, who, "a tensor is written over another one of the list");
   }
   return PL_OK;
 }
@@ -234,15 +240,13 @@ template <typename F> int for_each_piece(long n, const void* const* src, const l
   return flush();
 }
 
-int launch_status() { return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH; }
-
 // the norm's launches: partial sums into the workspace, *partials of them
 int launch_squares(long n, const void* const* src, const long long* counts, const int* types, double* workspace, int* partials, hipStream_t stream) {
   int used = 0;
   const int rc = for_each_piece(n, src, counts, types, nullptr, [&](const TensorList& list, int blocks) {
-    hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(NORM_THREADS), 0, stream, list, workspace + used);
+    double* const to = workspace + used;
     used += blocks;
-    return launch_status();
+    return launch(grad_squares_kernel, dim3(blocks), dim3(NORM_THREADS), stream, list, to);
   });
   *partials = used;
   return rc;
@@ -252,9 +256,9 @@ int launch_scale(long n, const void* const* src, const long long* counts, const 
                  const double* workspace, int partials, double* norm, hipStream_t stream) {
   int first = 1;
   return for_each_piece(n, src, counts, types, dst, [&](const TensorList& list, int blocks) {
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(blocks), dim3(NORM_THREADS), 0, stream, list, workspace, partials, first, max_norm, eps, norm);
+    const int store = first;
     first = 0;
-    return launch_status();
+    return launch(grad_scale_kernel, dim3(blocks), dim3(NORM_THREADS), stream, list, workspace, partials, store, max_norm, eps, norm);
   });
 }
 
@@ -270,8 +274,7 @@ int grad_norm_only(long n, const void* const* src, const long long* counts, cons
   int partials = 0;
   const int rc = launch_squares(n, src, counts, types, workspace, &partials, s);
   if (rc != PL_OK) return rc;
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(NORM_THREADS), 0, s, workspace, partials, norm);
-  return launch_status();
+  return launch(grad_norm_kernel, dim3(1), dim3(NORM_THREADS), s, workspace, partials, norm);
 }
 
 // no exception leaves a C entry: the checks' lists are the only thing that allocates

@@ -601,23 +601,22 @@ __global__ __launch_bounds__(WAVES * 64, 2) void half_few_columns_kernel(int M, 
 
 template <typename T, typename TD>
 int launch_few_columns(long M, long N, long K, const void* A, long lda, const void* B, long ldb, const Epilogue& ep, hipStream_t stream) {
-#define FEW(RB, NB, WAVES)                                                                                                                                         \
-  hipLaunchKernelGGL((half_few_columns_kernel<T, TD, RB, NB, WAVES>), dim3((unsigned)((M + 16 * RB - 1) / (16 * RB))), dim3(WAVES * 64), 0, stream, (int)M, (int)N, \
-                     (int)K, (const short*)A, lda, (const short*)B, ldb, ep)
+#define FEW(RB, NB, WAVES)                                                                                                                              \
+  return launch(half_few_columns_kernel<T, TD, RB, NB, WAVES>, dim3((unsigned)((M + 16 * RB - 1) / (16 * RB))), dim3(WAVES * 64), stream, (int)M, (int)N, \
+                (int)K, (const short*)A, lda, (const short*)B, ldb, ep)
   // One workgroup of eight waves per compute unit up to 256 of them; more come in fours, two to a unit, so that one's first
   // requests and its sums overlap the other's stream; 32 rows each where that still gives every unit two: half the reads of B.
   const long blocks = (M + 15) / 16;
-#define FEW_COLUMNS(NB)                  \
-  do {                                   \
-    if (blocks <= 256) FEW(1, NB, 8);    \
-    else if (blocks < 1024) FEW(1, NB, 4); \
-    else FEW(2, NB, 4);                  \
+#define FEW_COLUMNS(NB)                    \
+  do {                                     \
+    if (blocks <= 256) FEW(1, NB, 8);      \
+    if (blocks < 1024) FEW(1, NB, 4);      \
+    FEW(2, NB, 4);                         \
   } while (0)
   if (N <= 16) FEW_COLUMNS(1);
-  else FEW_COLUMNS(2);
+  FEW_COLUMNS(2);
 #undef FEW_COLUMNS
 #undef FEW
-  return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
 }
 
 // Rows of fewer than 8 elements (K < 8 of a K-major operand, M or N < 8 of an MN-major one) are no 16-byte vectors: a thread
@@ -641,21 +640,20 @@ int launch_half(const HalfPlan& plan, bool at, bool bt, bool padded, long M, lon
   const int gm = (int)((M + plan.tile - 1) / plan.tile), gn = (int)((N + plan.tile - 1) / plan.tile);
   const int fast = padded ? 3 : can_request(A, lda, B, ldb) ? 2 : in_offset_range(lda, ldb) ? 1 : 0;
 #define HALF(AKF, BKF, TILE, STAGES)                                                                                                                     \
-  hipLaunchKernelGGL((half_product_kernel<T, TD, AKF, BKF, TILE, TILE, STAGES, GRAD>), dim3(gm * gn, plan.splits), dim3(H_THREADS), 0, stream, (int)M, (int)N, \
-                     (int)K, (const short*)A, lda, (const short*)B, ldb, gm, gn, fast, plan.kchunk, ep)
+  return launch(half_product_kernel<T, TD, AKF, BKF, TILE, TILE, STAGES, GRAD>, dim3(gm * gn, plan.splits), dim3(H_THREADS), stream, (int)M, (int)N, (int)K, \
+                (const short*)A, lda, (const short*)B, ldb, gm, gn, fast, plan.kchunk, ep)
 #define HALF_TILE(TILE, STAGES)                    \
   do {                                             \
     if (at && !bt) HALF(true, true, TILE, STAGES); \
-    else if (at) HALF(true, false, TILE, STAGES);  \
-    else if (!bt) HALF(false, true, TILE, STAGES); \
-    else HALF(false, false, TILE, STAGES);         \
+    if (at) HALF(true, false, TILE, STAGES);       \
+    if (!bt) HALF(false, true, TILE, STAGES);      \
+    HALF(false, false, TILE, STAGES);              \
   } while (0)
   if (plan.tile == 256) HALF_TILE(256, 2);
-  else if (fast >= 2 && (long)gm * gn * plan.splits <= 256) HALF_TILE(128, 4);
-  else HALF_TILE(128, 2);
+  if (fast >= 2 && (long)gm * gn * plan.splits <= 256) HALF_TILE(128, 4);
+  HALF_TILE(128, 2);
 #undef HALF_TILE
 #undef HALF
-  return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
 }
 
 template <typename T, typename TD, bool GRAD>
@@ -670,9 +668,8 @@ int half_direct(const Call& c, const HalfPlan& plan, bool at, bool bt, const Epi
 template <typename T> int half_slices(const Call& c, const HalfPlan& plan, bool at, bool bt, void* slices) {
   if (plan.tile == 0) {
     const long blocks = (c.M * c.N + 255) / 256;
-    hipLaunchKernelGGL(half_thin_kernel<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, c.stream, c.M, c.N, (int)c.K, (const T*)c.A, at ? c.lda : 1L,
-                       at ? 1L : c.lda, (const T*)c.B, bt ? 1L : c.ldb, bt ? c.ldb : 1L, (float*)slices);
-    return hipGetLastError() == hipSuccess ? PL_OK : PL_ERR_LAUNCH;
+    return launch(half_thin_kernel<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), c.stream, c.M, c.N, (int)c.K, (const T*)c.A, at ? c.lda : 1L, at ? 1L : c.lda,
+                  (const T*)c.B, bt ? 1L : c.ldb, bt ? c.ldb : 1L, (float*)slices);
   }
   Epilogue plain = {};
   plain.alpha = 1.0;

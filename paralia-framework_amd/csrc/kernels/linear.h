@@ -5,11 +5,22 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "backend/pl_internal.h"
 #include "kernels/epilogue.h"
 #include "paralia_hip.h"
 
 namespace plk {
+
+// A launch without the triple-chevron's detour, arguments by reference: 128 tensors are 3.6 KB of them.
+template <typename... P>
+int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, const std::type_identity_t<P>&... args) {
+  void* list[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+  if (hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, 0, stream) == hipSuccess) return PL_OK;
+  (void)hipGetLastError();   // (reported here, not by the caller's next call)
+  return PL_ERR_LAUNCH;
+}
 
 inline bool valid_type(int t) { return t >= PL_TYPE_F64 && t <= PL_TYPE_BF16; }
 inline bool valid_act(int a) { return a >= PL_ACT_NONE && a <= PL_ACT_SILU; }
@@ -91,16 +102,20 @@ inline HalfPlan plan_half(bool at, bool bt, long M, long N, long K) {
   if ((at ? K : M) < 8 || (bt ? N : K) < 8) return {0, 1, 0};
   HalfPlan best = {128, 1, 0};
   double best_us = 1e30;
+  const unsigned k = (unsigned)K;
+  const double cells = (double)M * (double)N;
   for (const int tile : {128, 256}) {
     const long tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
-    for (int s = 1; s <= 32; ++s) {
-      const long kc = ((K + s - 1) / s + H_BK - 1) / H_BK * H_BK;
-      if (s > 1 && (kc < 2 * H_BK || (long)s * M * N * 4 > (256L << 20) || tiles * s > 2048)) break;
-      const long splits = s > 1 ? (K + kc - 1) / kc : 1;
-      if (splits != s) continue;
-      double us = 4.0 + half_rounds_us(tile, tiles * s, s > 1 ? (double)kc : (double)K);
-      if (s > 1) us += 4.0 + (4.0 * s + 4.0) * (double)M * (double)N / 4e6;
-      if (us < best_us * (s > 1 ? 0.95 : 1.0)) best_us = us, best = {tile, s, s > 1 ? (int)kc : 0};
+    for (const unsigned s : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 10u, 12u, 16u, 20u, 24u, 32u}) {
+      unsigned kc = k;
+      if (s > 1) {
+        kc = ((k + s - 1) / s + H_BK - 1) / H_BK * H_BK;
+        if (kc < 2 * H_BK || 4.0 * s * cells > (double)(256L << 20) || tiles * s > 2048) break;
+        if ((k + kc - 1) / kc != s) continue;
+      }
+      double us = 4.0 + half_rounds_us(tile, tiles * s, (double)kc);
+      if (s > 1) us += 4.0 + (4.0 * s + 4.0) * cells / 4e6;
+      if (us < best_us * (s > 1 ? 0.95 : 1.0)) best_us = us, best = {tile, (int)s, s > 1 ? (int)kc : 0};
     }
   }
   return best;

@@ -257,6 +257,23 @@ def test_alpha_zero_and_k_zero_do_not_read_the_operands(pkg, L, kind):
     assert torch.equal(got, bias[:, None].expand(M, N).to(TORCH[kind]).double())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(128, 1, 8192), (128, 130, 8192), (40, 3, 5), (700, 300, 1001)])
+def test_an_empty_gradient_stays_inside_its_workspace(pkg, L, kind, M, N, K):
+    """alpha = 0 where the product would be split, copied or thin: dZ = beta C act'(Z), its sums, and nothing behind the
+    workspace."""
+    Cm, Z = rand_ints(M, N, 1, -9, 9), rand_ints(M, N, 2, -3, 3)
+    Cb, Zb, D, db = Mat(M, N, M, kind).set(Cm), Mat(M, N, M, kind).set(Z), Mat(M, N, M, kind, gap=7.0), Mat(M, 1, M, kind, gap=5.0)
+    need = L.pl_gemm_epilogue_workspace_bytes(TYPES[kind], b"N", b"N", M, N, K, 1)
+    ws = torch.full((need + 8192,), 0xA5, dtype=torch.uint8, device="cuda")
+    pkg.check(L.pl_gemm_epilogue_grad(TYPES[kind], b"N", b"N", M, N, K, 0.0, None, M, None, K, ACTS["relu"], Zb.ptr, M, 2.0, Cb.ptr, M, D.ptr, M, db.ptr, ws.data_ptr(), need,
+                                      torch.cuda.current_stream().cuda_stream), "pl_gemm_epilogue_grad")
+    torch.cuda.synchronize()
+    want = 2.0 * Cm * (Z > 0)
+    assert torch.equal(D.get(), want) and torch.equal(db.get()[:, 0], want.sum(1).to(TORCH[kind]).double())
+    assert bool((ws[need:] == 0xA5).all())
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_row_ranges_of_larger_matrices(pkg, L, kind):
     """Operands and results that are row ranges of packed buffers (three projections side by side): only the named rows
