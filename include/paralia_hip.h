@@ -267,7 +267,7 @@ int pl_gemm_epilogue_grad(int type, char transA, char transB, long M, long N, lo
  * and activation where dY is an operand.  dZ may be dY or Z itself, or null where only dbias is wanted; dbias may be
  * null.  N == 0 leaves a dbias of zeros.  workspace (only with dbias): pl_bias_act_grad_workspace_bytes bytes, 16-byte
  * aligned.  The order of the sums depends only on the shape and the type, here and
- * above (there, with 16-bit operands, also on whether they can be requested). */
+ * above (there also on whether the operands are 16-byte aligned). */
 long pl_bias_act_grad_workspace_bytes(int type, long M, long N);
 int pl_bias_act_grad(int type, int activation, long M, long N, const void* dY, long lddy, const void* Z, long ldz, void* dZ, long lddz,
                      void* dbias, void* workspace, long workspace_bytes, void* stream);

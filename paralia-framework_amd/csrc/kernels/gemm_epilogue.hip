@@ -8,10 +8,10 @@
 
 namespace plk {
 
-// The workspace of one call, in the order it is laid out: the product or its slices, the partial bias gradients, aligned copies of 16-bit operands.
+// The workspace of one call, in the order it is laid out: the product or its slices, the partial bias gradients, aligned copies of the operands.
 struct Workspace { long product, partial, copies; long bytes() const { return product + partial + copies; } };
 inline long round16(long b) { return (b + 15) & ~15L; }
-inline Workspace workspace_for(int type, const HalfPlan& p, const HalfCopies& copies, bool at, bool bt, long M, long N, long K, bool dbias) {
+inline Workspace workspace_for(int type, const HalfPlan& p, const Copies& copies, bool at, bool bt, long M, long N, long K, bool dbias) {
   Workspace w = {0, 0, 0};
   const long wide = type == PL_TYPE_F64 ? 8 : 4;
   if (type_size(type) == 2) {
@@ -22,19 +22,26 @@ inline Workspace workspace_for(int type, const HalfPlan& p, const HalfCopies& co
       const long tile_rows = half_partial_rows({128, 1, 0}, type, M, N), pass_rows = half_partial_rows({0, 1, 0}, type, M, N);
       w.partial = round16((tile_rows > pass_rows ? tile_rows : pass_rows) * M * wide);
     }
-    w.copies = copies.bytes();
   } else {
-    // the slices of a product alone on the device, or the product and behind it the slices of its tail
-    w.product = round16(M * N * wide) + round16(pl_gemm_tile_alone_workspace_bytes(at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, type_size(type)));
+    // the slices of a product alone on the device, or the product and behind it the slices of its tail; of the operands and
+    // of their copies, whichever the call will be given
+    const char ta = at ? 'T' : 'N', tb = bt ? 'T' : 'N';
+    long slices = pl_gemm_tile_alone_workspace_bytes(ta, tb, M, N, K, 1, (int)wide);
+    if (copies.bytes() > 0) {
+      const long padded = pl_gemm_tile_alone_workspace_bytes(ta, tb, M, N, whole(K, WIDE_K), 1, (int)wide);
+      if (padded > slices) slices = padded;
+    }
+    w.product = round16(M * N * wide) + round16(slices);
     if (dbias) w.partial = round16(epilogue_pass_rows(type, M, N) * M * wide);
   }
+  w.copies = copies.bytes();
   return w;
 }
 
-// blockIdx.y: which operand.  `rows` rows of `extent` elements into `rows_to` rows of ld_to, zeros behind them.
-struct HalfCopyJob { const short* from; short* to; long ld, ld_to, rows, rows_to; int extent; };
-__global__ __launch_bounds__(256) void half_copy_kernel(HalfCopyJob a, HalfCopyJob b) {
-  const HalfCopyJob j = blockIdx.y == 0 ? a : b;
+// blockIdx.y: which operand.  `rows` rows of `extent` pairs of bytes into `rows_to` rows of ld_to, zeros behind them.
+struct CopyJob { const short* from; short* to; long ld, ld_to, rows, rows_to; int extent; };
+__global__ __launch_bounds__(256) void copy_kernel(CopyJob a, CopyJob b) {
+  const CopyJob j = blockIdx.y == 0 ? a : b;
   const long per_row = j.ld_to / 8, total = per_row * j.rows_to;
   typedef Loose<short>::vec vec;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
@@ -53,12 +60,13 @@ __global__ __launch_bounds__(256) void half_copy_kernel(HalfCopyJob a, HalfCopyJ
     *reinterpret_cast<vec*>(j.to + row * j.ld_to + at) = v;
   }
 }
-int half_copy(const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const HalfCopies& to) {
-  const HalfCopyJob a = {(const short*)A, (short*)copy_a, lda, to.ld_a, at ? c.M : c.K, to.bytes_a / (2 * to.ld_a), (int)(at ? c.K : c.M)};
-  const HalfCopyJob b = {(const short*)B, (short*)copy_b, ldb, to.ld_b, bt ? c.K : c.N, to.bytes_b / (2 * to.ld_b), (int)(bt ? c.N : c.K)};
+int copy_operands(int es, const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const Copies& to) {
+  const long u = es / 2;
+  const CopyJob a = {(const short*)A, (short*)copy_a, lda * u, to.ld_a * u, at ? c.M : c.K, to.bytes_a / (es * to.ld_a), (int)((at ? c.K : c.M) * u)};
+  const CopyJob b = {(const short*)B, (short*)copy_b, ldb * u, to.ld_b * u, bt ? c.K : c.N, to.bytes_b / (es * to.ld_b), (int)((bt ? c.N : c.K) * u)};
   const long most = (to.bytes_a > to.bytes_b ? to.bytes_a : to.bytes_b) / 16;
   const long blocks = (most + 255) / 256;
-  return launch(half_copy_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), c.stream, a, b);
+  return launch(copy_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), c.stream, a, b);
 }
 
 bool plain_product(const Call& c) {
@@ -100,10 +108,11 @@ int run_product(Call& c) {
   if (!same_or_apart(d, rc) || !same_or_apart(d, z)) return refuse(PL_ERR_ARG, who, "D overlaps C or Z without being it");
   const bool few = es == 2 && !empty && few_columns(c, at, bt);   // (a kernel that needs no workspace, and no plan)
   HalfPlan plan = {0, 1, 0};
-  HalfCopies copies = {0, 0, 0, 0};
+  Copies copies = {0, 0, 0, 0};
   Workspace w = {0, 0, 0};
   if (!few) {
-    if (es == 2) plan = plan_half(at, bt, M, N, K), copies = half_copies(at, bt, M, N, K);
+    if (es == 2) plan = plan_half(at, bt, M, N, K);
+    copies = es == 2 ? half_copies(at, bt, M, N, K) : wide_copies(es, false, at, bt, M, N, K);
     w = workspace_for(c.type, plan, copies, at, bt, M, N, K, c.dbias != nullptr);
   }
   if (w.bytes() > 0 && (!c.workspace || !aligned_to(c.workspace, 16) || c.workspace_bytes < w.bytes())) return refuse(PL_ERR_ARG, who, "workspace null, too small or not 16-byte aligned");
@@ -115,18 +124,21 @@ int run_product(Call& c) {
   ep.partial = c.dbias ? ws + w.product : nullptr;
   if (empty) c.K = 0;
   int rc_;
-  long rows;
+  long rows, m_read = M, n_read = N;
+  const bool copied = es == 2 ? !can_request(c.A, c.lda, c.B, c.ldb) && in_offset_range(copies.ld_a, copies.ld_b)
+                              : wide_copies(es, wide_aligned(es, c.A, c.lda, c.B, c.ldb), at, bt, M, N, K).bytes() > 0;
+  if (!empty && copies.bytes() > 0 && copied) {
+    char* const copy_a = ws + w.product + w.partial;
+    rc_ = copy_operands(es, c.A, c.lda, copy_a, c.B, c.ldb, copy_a + copies.bytes_a, c, at, bt, copies);
+    if (rc_ != PL_OK) return rc_;
+    c.A = copy_a, c.lda = copies.ld_a;
+    c.B = copy_a + copies.bytes_a, c.ldb = copies.ld_b;
+    c.K = whole(K, es == 2 ? H_BK : WIDE_K);
+    c.padded = true;
+    m_read = whole(M, WIDE_ROWS), n_read = whole(N, WIDE_ROWS);
+  }
   if (es == 2) {
     if (empty) plan.splits = 1, plan.kchunk = 0;
-    if (!empty && copies.bytes() > 0 && !can_request(c.A, c.lda, c.B, c.ldb) && in_offset_range(copies.ld_a, copies.ld_b)) {
-      char* const copy_a = ws + w.product + w.partial;
-      rc_ = half_copy(c.A, c.lda, copy_a, c.B, c.ldb, copy_a + copies.bytes_a, c, at, bt, copies);
-      if (rc_ != PL_OK) return rc_;
-      c.A = copy_a, c.lda = copies.ld_a;
-      c.B = copy_a + copies.bytes_a, c.ldb = copies.ld_b;
-      c.K = (K + H_BK - 1) / H_BK * H_BK;
-      c.padded = true;
-    }
     if (plan.tile == 256 && !can_request(c.A, c.lda, c.B, c.ldb)) plan.tile = 128;
     rows = few ? 0 : half_partial_rows(plan, c.type, M, N);
     const bool f16 = c.type == PL_TYPE_F16, sliced = !few && (plan.tile == 0 || plan.splits > 1);
@@ -145,11 +157,11 @@ int run_product(Call& c) {
     const bool f64 = c.type == PL_TYPE_F64;
     if (plain_product(c)) {
       // nothing but the product (and C where D is): the tile GEMM's own epilogue
-      return f64 ? pl_dgemm_tile_alone(c.ta, c.tb, M, N, c.K, ep.alpha, (const double*)c.A, c.lda, (const double*)c.B, c.ldb, ep.beta, (double*)ep.D, ep.ldd, ws, w.product, c.stream)
-                 : pl_sgemm_tile_alone(c.ta, c.tb, M, N, c.K, (float)ep.alpha, (const float*)c.A, c.lda, (const float*)c.B, c.ldb, (float)ep.beta, (float*)ep.D, ep.ldd, ws, w.product, c.stream);
+      return f64 ? pl_dgemm_tile_padded(c.ta, c.tb, M, N, c.K, ep.alpha, (const double*)c.A, c.lda, (const double*)c.B, c.ldb, ep.beta, (double*)ep.D, ep.ldd, ws, w.product, -1, m_read, n_read, c.stream)
+                 : pl_sgemm_tile_padded(c.ta, c.tb, M, N, c.K, (float)ep.alpha, (const float*)c.A, c.lda, (const float*)c.B, c.ldb, (float)ep.beta, (float*)ep.D, ep.ldd, ws, w.product, -1, m_read, n_read, c.stream);
     }
     int slices = 1;
-    rc_ = (f64 ? product_slices_f64 : product_slices_f32)(c.ta, c.tb, M, N, c.K, c.A, c.lda, c.B, c.ldb, ws, w.product, f64 && c.grad, &slices, c.stream);
+    rc_ = (f64 ? product_slices_f64 : product_slices_f32)(c.ta, c.tb, M, N, c.K, c.A, c.lda, c.B, c.ldb, ws, w.product, m_read, n_read, f64 && c.grad, &slices, c.stream);
     if (rc_ == PL_OK) rc_ = epilogue_pass(c.type, c.type_d, c.grad, M, N, ws, M, M * N, slices, ep, c.stream);
   }
   if (rc_ != PL_OK || !c.dbias) return rc_;
@@ -162,8 +174,9 @@ extern "C" long pl_gemm_epilogue_workspace_bytes(int type, char transA, char tra
   using namespace plk;
   if (!valid_type(type) || M <= 0 || N <= 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
   const bool at = transA == 'T' || transA == 't', bt = transB == 'T' || transB == 't';
-  const bool half = type_size(type) == 2;
-  return workspace_for(type, half ? plan_half(at, bt, M, N, K) : HalfPlan{0, 1, 0}, half ? half_copies(at, bt, M, N, K) : HalfCopies{0, 0, 0, 0}, at, bt, M, N, K, with_dbias != 0).bytes();
+  const int es = type_size(type);
+  const HalfPlan plan = es == 2 ? plan_half(at, bt, M, N, K) : HalfPlan{0, 1, 0};
+  return workspace_for(type, plan, es == 2 ? half_copies(at, bt, M, N, K) : wide_copies(es, false, at, bt, M, N, K), at, bt, M, N, K, with_dbias != 0).bytes();
 }
 
 extern "C" int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda, const void* B, long ldb,

@@ -1232,20 +1232,23 @@ int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, l
 // For a caller that finishes the product itself (the fused epilogue of the linear layers): op(A) * op(B) as a product alone
 // on the device would run it, into `slices` dense M x N slices at ws that are still to be added (1, or add: the product itself).
 template <typename T>
-int product_slices(char ta, char tb, long M, long N, long K, const T* A, long lda, const T* B, long ldb, T* ws, long ws_bytes, bool add, int* slices, hipStream_t stream) {
+int product_slices(char ta, char tb, long M, long N, long K, const T* A, long lda, const T* B, long ldb, T* ws, long ws_bytes, long m_read, long n_read,
+                   bool add, int* slices, hipStream_t stream) {
   const bool an = ta == 'N' || ta == 'n', bnn = tb == 'N' || tb == 'n';
-  *slices = K > 0 ? choose_tile<T>(an, bnn, M, N, K, true, true, ws_bytes, true, 0, true).splits : 1;
+  *slices = K > 0 ? choose_tile<T>(an, bnn, M, N, K, true, true, ws_bytes, true, 0, true, m_read, n_read).splits : 1;
   if (add) *slices = 1;
-  if (*slices > 1) return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, ws, ws_bytes, *slices, false, 0, 0, false, true);
+  if (*slices > 1) return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, ws, ws_bytes, *slices, false, m_read, n_read, false, true);
   // one launch, or an unsplit head and a split tail whose slices lie behind the product
   const long product = (M * N * (long)sizeof(T) + 15) & ~15L;
-  return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, (T*)((char*)ws + product), ws_bytes - product, 0, true);
+  return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, (T*)((char*)ws + product), ws_bytes - product, 0, true, m_read, n_read);
 }
-int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream) {
-  return product_slices<float>(ta, tb, M, N, K, (const float*)A, lda, (const float*)B, ldb, (float*)ws, ws_bytes, add, slices, stream);
+int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
+                       int* slices, hipStream_t stream) {
+  return product_slices<float>(ta, tb, M, N, K, (const float*)A, lda, (const float*)B, ldb, (float*)ws, ws_bytes, m_read, n_read, add, slices, stream);
 }
-int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream) {
-  return product_slices<double>(ta, tb, M, N, K, (const double*)A, lda, (const double*)B, ldb, (double*)ws, ws_bytes, add, slices, stream);
+int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
+                       int* slices, hipStream_t stream) {
+  return product_slices<double>(ta, tb, M, N, K, (const double*)A, lda, (const double*)B, ldb, (double*)ws, ws_bytes, m_read, n_read, add, slices, stream);
 }
 
 template <typename T>

@@ -61,8 +61,10 @@ inline bool same_or_apart(const Range& a, const Range& b) {
 }
 
 // gemm_mfma.hip: the fp32 / fp64 product in slices that are still to be added
-int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream);
-int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, bool add, int* slices, hipStream_t stream);
+int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
+                       int* slices, hipStream_t stream);
+int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
+                       int* slices, hipStream_t stream);
 
 // epilogue.hip
 int bias_fold(int type, long M, long rows, const void* partial, void* dbias, hipStream_t stream);
@@ -138,23 +140,49 @@ inline bool can_request(const void* A, long lda, const void* B, long ldb) {
 // panels are loaded by every tile in its row or column, and the copies cost one launch and one pass over the operands
 // (4100 x 1023 x 2052, rows of an odd number of elements: 70 -> 47 us).  The space is set aside by the shape alone: where a
 // contiguous extent is no multiple of 8, so that dense operands could not be aligned.
-struct HalfCopies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
-inline HalfCopies half_copies(bool at, bool bt, long M, long N, long K) {
+inline long whole(long n, long unit) { return (n + unit - 1) / unit * unit; }
+struct Copies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
+inline Copies half_copies(bool at, bool bt, long M, long N, long K) {
   const long ext_a = at ? K : M, rows_a = at ? M : K, ext_b = bt ? N : K, rows_b = bt ? K : N;
-  HalfCopies c = {0, 0, 0, 0};
+  Copies c = {0, 0, 0, 0};
   if ((ext_a % 8 == 0 && ext_b % 8 == 0) || ext_a < 8 || ext_b < 8 || K > (1L << 30)) return c;
   const double tiles = (double)((M + 127) / 128) * (double)((N + 127) / 128);
   const double slow_us = 0.8 * (double)(K / H_BK) * (tiles > 256.0 ? tiles / 256.0 : 1.0), copy_us = 6.0 + 4.0 * (double)K * (double)(M + N) / 3e6;
   if (slow_us < copy_us) return c;
   // rows in whole cache lines, and k filled up with zeros to whole panels in either layout
-  auto whole = [](long n) { return (n + H_BK - 1) / H_BK * H_BK; };
-  c.ld_a = whole(ext_a);
-  c.ld_b = whole(ext_b);
-  c.bytes_a = (at ? rows_a : whole(rows_a)) * c.ld_a * 2;
-  c.bytes_b = (bt ? whole(rows_b) : rows_b) * c.ld_b * 2;
+  c.ld_a = whole(ext_a, H_BK);
+  c.ld_b = whole(ext_b, H_BK);
+  c.bytes_a = (at ? rows_a : whole(rows_a, H_BK)) * c.ld_a * 2;
+  c.bytes_b = (bt ? whole(rows_b, H_BK) : rows_b) * c.ld_b * 2;
   return c;
 }
-int half_copy(const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const HalfCopies& to);
+
+// The same for fp32 and fp64, whose tile GEMM takes panels straight into LDS only from 16-byte aligned vectors and only in
+// whole tiles and panels: from aligned copies with k filled up by zeros to whole panels and rows to whole tiles of 256, an
+// unaligned product runs at nearly the full rate (3878 x 1869 x 4113 with odd strides, fp32 TN / NN / NT / TT: 970 / 900 /
+// 781 / 900 -> 537 / 506 / 507 / 506 us, fp64 1092 - 1190 -> 1010 - 1080), and of aligned operands with ragged edges loses
+// less (3880 x 1872 x 4112: fp32 551 - 598 -> 504, fp64 1076 - 1130 -> 1000 - 1010).  Products that fill less of the device
+// lose less; below the copies' own time there are none.  The space is set aside for whole extents too: their rows may be
+// those of a wider matrix.
+constexpr long WIDE_ROWS = 256, WIDE_K = 32;
+inline bool wide_aligned(int es, const void* A, long lda, const void* B, long ldb) {
+  return aligned_to(A, 16) && aligned_to(B, 16) && lda % (16 / es) == 0 && ldb % (16 / es) == 0;
+}
+inline Copies wide_copies(int es, bool aligned, bool at, bool bt, long M, long N, long K) {
+  Copies c = {0, 0, 0, 0};
+  if (K <= 0 || M > (1L << 28) || N > (1L << 28) || K > (1L << 28)) return c;
+  const bool ragged = M % 128 != 0 || N % 128 != 0 || K % WIDE_K != 0;
+  const double product_us = 2.0 * (double)M * (double)N * (double)K / (es == 4 ? 138e6 : 72e6);
+  const double gain = !aligned ? (es == 4 ? 0.6 : 0.25) : ragged ? (es == 4 ? 0.15 : 0.1) : 0.0;
+  const long kw = whole(K, WIDE_K), mw = whole(M, WIDE_ROWS), nw = whole(N, WIDE_ROWS);
+  if (gain * product_us < 10.0 + (double)es * (double)kw * (double)(2 * mw + 2 * nw) / 3e6) return c;
+  c.ld_a = at ? kw : mw;
+  c.ld_b = bt ? nw : kw;
+  c.bytes_a = (at ? mw : kw) * c.ld_a * es;
+  c.bytes_b = (bt ? kw : nw) * c.ld_b * es;
+  return c;
+}
+int copy_operands(int es, const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const Copies& to);
 
 // few columns of two K-major operands that can be requested, in whole panels of k: a kernel of their own
 constexpr int FEW_MAX_N = 32;

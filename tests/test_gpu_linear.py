@@ -363,8 +363,24 @@ def test_wide_products_split_and_cut(pkg, L, kind, ta, tb, M, N, K):
     assert torch.equal(got, want) and torch.equal(db, want.sum(1))
 
 
+@pytest.mark.parametrize("kind,M,N,K", [("f32", 1501, 1301, 2003), ("f32", 3000, 130, 8192), ("f32", 8193, 2050, 257), ("f64", 2501, 2001, 2003), ("f64", 1280, 5001, 1536)])
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_wide_products_of_unaligned_operands(pkg, L, kind, ta, tb, M, N, K):
+    """Large enough to be multiplied from aligned copies: ragged extents, and whole ones in rows of an odd stride."""
+    for lay in (Layout(pad=1), Layout(pad=3, offset=1)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay)
+    opA, opB, Cm = rand_ints(M, K, 7), rand_ints(K, N, 8), rand_ints(M, N, 9, -9, 9)
+    got, _ = product(pkg, L, kind, ta, tb, opA, opB, alpha=2.0, beta=-1.0, Cm=Cm, in_place=True, lay=Layout(pad=1))
+    assert torch.equal(got, 2.0 * (opA @ opB) - Cm)
+    opA, opB, Z = rand(M, K, 31, kind, K ** -0.5), rand(K, N, 32, kind), rand(M, N, 33, kind, 2.0)
+    d, ed, db, edb = gradient(opA, opB, Z, None, 1.0, 0.0, "gelu_tanh", kind)
+    got, gdb = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="gelu_tanh", lay=Layout(pad=1))
+    check(got, d, ed, "D")
+    check(gdb, db, edb, "dbias")
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("ta,tb,M,N,K", [("T", "N", 700, 300, 1001), ("N", "N", 256, 256, 4096), ("N", "T", 300, 200, 64), ("T", "T", 3, 5, 9)])
+@pytest.mark.parametrize("ta,tb,M,N,K", [("T", "N", 700, 300, 1001), ("N", "N", 256, 256, 4096), ("N", "T", 300, 200, 64), ("T", "T", 3, 5, 9), ("N", "N", 2051, 1701, 2003)])
 def test_nothing_is_written_behind_the_workspace(pkg, L, kind, ta, tb, M, N, K):
     opA, opB, Z = rand_ints(M, K, 1), rand_ints(K, N, 2), rand_ints(M, N, 3)
     A, B = Mat(*((M, K) if ta == "N" else (K, M)), M if ta == "N" else K, kind).set(opA if ta == "N" else opA.T), Mat(*((K, N) if tb == "N" else (N, K)), K if tb == "N" else N, kind).set(opB if tb == "N" else opB.T)
