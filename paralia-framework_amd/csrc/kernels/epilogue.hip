@@ -35,6 +35,7 @@ __global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, lon
       W v[VEC];
       load_row<TP, VEC, W>(P + n * ldP + m, v, valid);
       if constexpr (SLICES) {
+#pragma unroll 4
         for (int s = 1; s < slices; ++s) {
           W x[VEC];
           load_row<TP, VEC, W>(P + s * slice + n * ldP + m, x, valid);

@@ -11,7 +11,7 @@ namespace plk {
 // The workspace of one call, in the order it is laid out: the product or its slices, the partial bias gradients, aligned copies of the operands.
 struct Workspace { long product, partial, copies; long bytes() const { return product + partial + copies; } };
 inline long round16(long b) { return (b + 15) & ~15L; }
-inline Workspace workspace_for(int type, const HalfPlan& p, const Copies& copies, bool at, bool bt, long M, long N, long K, bool dbias) {
+inline Workspace workspace_for(int type, const HalfPlan& p, const WidePlan& wp, const Copies& copies, bool at, bool bt, long M, long N, long K, bool dbias) {
   Workspace w = {0, 0, 0};
   const long wide = type == PL_TYPE_F64 ? 8 : 4;
   if (type_size(type) == 2) {
@@ -22,6 +22,10 @@ inline Workspace workspace_for(int type, const HalfPlan& p, const Copies& copies
       const long tile_rows = half_partial_rows({128, 1, 0}, type, M, N), pass_rows = half_partial_rows({0, 1, 0}, type, M, N);
       w.partial = round16((tile_rows > pass_rows ? tile_rows : pass_rows) * M * wide);
     }
+  } else if (wp.splits > 0) {
+    if (wp.splits > 1) w.product = round16((long)wp.splits * M * N * wide);
+    const long tile_rows = (N + 63) / 64, pass_rows = epilogue_pass_rows(type, M, N);   // (the larger, as above)
+    if (dbias) w.partial = round16((tile_rows > pass_rows ? tile_rows : pass_rows) * M * wide);
   } else {
     // the slices of a product alone on the device, or the product and behind it the slices of its tail; of the operands and
     // of their copies, whichever the call will be given
@@ -108,12 +112,13 @@ int run_product(Call& c) {
   if (!same_or_apart(d, rc) || !same_or_apart(d, z)) return refuse(PL_ERR_ARG, who, "D overlaps C or Z without being it");
   const bool few = es == 2 && !empty && few_columns(c, at, bt);   // (a kernel that needs no workspace, and no plan)
   HalfPlan plan = {0, 1, 0};
+  WidePlan tiles = {0, 0};
   Copies copies = {0, 0, 0, 0};
   Workspace w = {0, 0, 0};
   if (!few) {
-    if (es == 2) plan = plan_half(at, bt, M, N, K);
-    copies = es == 2 ? half_copies(at, bt, M, N, K) : wide_copies(es, false, at, bt, M, N, K);
-    w = workspace_for(c.type, plan, copies, at, bt, M, N, K, c.dbias != nullptr);
+    if (es == 2) plan = plan_half(at, bt, M, N, K), copies = half_copies(at, bt, M, N, K);
+    else if (tiles = plan_wide(es, at, bt, M, N, K); tiles.splits == 0) copies = wide_copies(es, false, at, bt, M, N, K);
+    w = workspace_for(c.type, plan, tiles, copies, at, bt, M, N, K, c.dbias != nullptr);
   }
   if (w.bytes() > 0 && (!c.workspace || !aligned_to(c.workspace, 16) || c.workspace_bytes < w.bytes())) return refuse(PL_ERR_ARG, who, "workspace null, too small or not 16-byte aligned");
   const Range work = bytes_at(w.bytes() > 0 ? c.workspace : nullptr, w.bytes());
@@ -152,6 +157,10 @@ int run_product(Call& c) {
     } else {
       rc_ = f16 ? half_forward_f16(c, plan, at, bt, ep) : half_forward_bf16(c, plan, at, bt, ep);
     }
+  } else if (tiles.splits > 0) {
+    if (empty) tiles.splits = 1;
+    rows = tiles.splits > 1 ? epilogue_pass_rows(c.type, M, N) : (N + 63) / 64;
+    rc_ = (es == 8 ? wide_product_f64 : wide_product_f32)(c, tiles, at, bt, ep, ws);
   } else {
     rows = epilogue_pass_rows(c.type, M, N);
     const bool f64 = c.type == PL_TYPE_F64;
@@ -176,7 +185,9 @@ extern "C" long pl_gemm_epilogue_workspace_bytes(int type, char transA, char tra
   const bool at = transA == 'T' || transA == 't', bt = transB == 'T' || transB == 't';
   const int es = type_size(type);
   const HalfPlan plan = es == 2 ? plan_half(at, bt, M, N, K) : HalfPlan{0, 1, 0};
-  return workspace_for(type, plan, es == 2 ? half_copies(at, bt, M, N, K) : wide_copies(es, false, at, bt, M, N, K), at, bt, M, N, K, with_dbias != 0).bytes();
+  const WidePlan tiles = es == 2 ? WidePlan{0, 0} : plan_wide(es, at, bt, M, N, K);
+  const Copies copies = es == 2 ? half_copies(at, bt, M, N, K) : tiles.splits > 0 ? Copies{0, 0, 0, 0} : wide_copies(es, false, at, bt, M, N, K);
+  return workspace_for(type, plan, tiles, copies, at, bt, M, N, K, with_dbias != 0).bytes();
 }
 
 extern "C" int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda, const void* B, long ldb,

@@ -87,6 +87,8 @@ struct Call {
   hipStream_t stream;
 };
 
+inline long whole(long n, long unit) { return (n + unit - 1) / unit * unit; }
+
 constexpr int H_BK = 64;   // panel depth of the 16-bit product
 
 // How a 16-bit product is launched: macro tile, and how many ways K is split so that few tiles still fill the chip.  A
@@ -128,6 +130,42 @@ inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
   return p.splits > 1 || p.tile == 0 ? epilogue_pass_rows(type, M, N) : 2 * ((N + p.tile - 1) / p.tile);
 }
 
+// How an fp32 or fp64 product is launched: in the tile GEMM's tiles with the epilogue as a pass (splits 0), or in 64 x 64 tiles
+// with the epilogue inside, K split `splits` ways where it is long.  A function of the shape and the type alone.  Times in
+// microseconds, fitted to 156 products of 64 x 64 x 64 to 8192 x 2048 x 2048: a 64 x 64 tile alone on its unit takes 0.053
+// (fp32 0.032) per k, several on one 0.039 (0.0245) each, and 2 (1) for its epilogue; a pass over slices 3, 0.8 for each slice
+// and their bytes at 4 TB/s.  The rule's choices are 2 % from the best of all measured ones, the tile GEMM's 26 %.
+// Both sides, fp64 / fp32, tile GEMM -> 64 x 64: 605 x 195 x 174 38 / 30 -> 17 / 11, 9472 x 192 x 3 21 / 17 -> 11 / 9,
+// 10474 x 17 x 2943 170 / 105 -> 99 / 69; 2048 x 2048 x 512 79 / 44 -> 87 / 54, 2048^3 256 / 133 -> 318 / 192.
+struct WidePlan { int splits, kchunk; };
+inline WidePlan plan_wide(int es, bool at, bool bt, long M, long N, long K) {
+  if (M > (1L << 27) || N > (1L << 27) || K > (1L << 30)) return {0, 0};
+  const double cells_us = (double)M * (double)N * es / 4e6, lone = es == 8 ? 0.053 : 0.032, shared = es == 8 ? 0.039 : 0.0245;
+  const long tiles = ((M + 63) / 64) * ((N + 63) / 64);
+  const int k = (int)K, gran = 128 / es;
+  WidePlan best = {1, 0};
+  double best_us = 1e30;
+  for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    int kc = k;
+    if (s > 1) {
+      kc = ((k + s - 1) / s + gran - 1) / gran * gran;
+      if (kc < 2 * gran || s * cells_us > 64.0) break;
+      if ((k + kc - 1) / kc != s) continue;
+    }
+    const double per_unit = (double)((tiles * s + 255) / 256);
+    double us = 5.5 + (lone > per_unit * shared ? lone : per_unit * shared) * kc + per_unit * (0.25 * es) + 0.5 * cells_us;
+    if (s > 1) us += 3.0 + 0.8 * s + 2.0 * s * cells_us;
+    if (us < best_us * (s > 1 ? 0.95 : 1.0)) best_us = us, best = {s, s > 1 ? kc : 0};
+  }
+  if (best_us < 10.0 || K == 0) return best;   // (less than the tile GEMM's two launches ever take)
+  const long per = 16 / es;
+  const bool unaligned = (at ? K : M) % per != 0 || (bt ? N : K) % per != 0, ragged = M % 128 != 0 || N % 128 != 0 || K % 32 != 0;
+  const double gemm = pl_gemm_tile_alone_us(es, at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, 1L << 28) * (unaligned ? (es == 4 ? 1.6 : 1.25) : ragged ? 1.1 : 1.0);
+  return best_us < 0.95 * (5.0 + gemm + 2.0 * cells_us) ? best : WidePlan{0, 0};
+}
+int wide_product_f32(const Call& c, const WidePlan& plan, bool at, bool bt, const Epilogue& ep, void* slices);
+int wide_product_f64(const Call& c, const WidePlan& plan, bool at, bool bt, const Epilogue& ep, void* slices);
+
 // requests: 16-byte granules, and offsets from a panel's first element in 32 bits (256 rows of a K-major operand, 64 k-rows
 // of an MN-major one)
 inline bool in_offset_range(long lda, long ldb) { return lda < (1L << 22) && ldb < (1L << 22); }
@@ -140,7 +178,6 @@ inline bool can_request(const void* A, long lda, const void* B, long ldb) {
 // panels are loaded by every tile in its row or column, and the copies cost one launch and one pass over the operands
 // (4100 x 1023 x 2052, rows of an odd number of elements: 70 -> 47 us).  The space is set aside by the shape alone: where a
 // contiguous extent is no multiple of 8, so that dense operands could not be aligned.
-inline long whole(long n, long unit) { return (n + unit - 1) / unit * unit; }
 struct Copies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
 inline Copies half_copies(bool at, bool bt, long M, long N, long K) {
   const long ext_a = at ? K : M, rows_a = at ? M : K, ext_b = bt ? N : K, rows_b = bt ? K : N;
