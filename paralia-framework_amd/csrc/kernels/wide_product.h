@@ -18,6 +18,7 @@ namespace plk {
 template <typename T> struct WideTile {
   static constexpr int BK = 128 / (int)sizeof(T);      // panel depth
   static constexpr int LOADS = 64 * BK / 256;          // elements a thread loads of each operand's panel
+  static constexpr int AHEAD = 2;                      // panels in flight (even: two buffers take turns; four are no faster)
   static constexpr int PITCH = 80;
   static constexpr int VEC = 16 / (int)sizeof(T);
   static constexpr int TILE_PITCH = sizeof(T) == 8 ? 80 : 68;   // the product on its way to the epilogue: 16 rows of 4 columns at once
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(256, 3) void wide_tile_kernel(int M, int N, int K, 
     for (int j = 0; j < 2; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
   const WideOperand<T, AK> a(A, lda, m0, M, tid);
   const WideOperand<T, BKM> b(B, ldb, n0, N, tid);
-  T ra[2][S::LOADS], rb[2][S::LOADS];
+  T ra[S::AHEAD][S::LOADS], rb[S::AHEAD][S::LOADS];
   const int i16 = lane & 15, g = lane >> 4, wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
   auto panel = [&](T (&pa)[S::LOADS], T (&pb)[S::LOADS], int k0, int half) {
     T* const la = lds + half * 2 * BK * S::PITCH;
@@ -98,8 +99,8 @@ __global__ __launch_bounds__(256, 3) void wide_tile_kernel(int M, int N, int K, 
     b.store(pb, lb, k0, k_last);
     // (the panel before last was multiplied before the barrier that its successor's writers passed: this half is free)
     __syncthreads();
-    a.load(pa, k0 + 2 * BK, k_last);
-    b.load(pb, k0 + 2 * BK, k_last);
+    a.load(pa, k0 + S::AHEAD * BK, k_last);
+    b.load(pb, k0 + S::AHEAD * BK, k_last);
 #pragma unroll
     for (int s = 0; s < BK / 4; ++s) {
       const int k = 4 * s + g, at = k * S::PITCH + (i16 ^ S::turn(k));
@@ -113,14 +114,14 @@ __global__ __launch_bounds__(256, 3) void wide_tile_kernel(int M, int N, int K, 
     }
   };
   if (k_first <= k_last) {
-    a.load(ra[0], k_first, k_last);
-    b.load(rb[0], k_first, k_last);
-    a.load(ra[1], k_first + BK, k_last);
-    b.load(rb[1], k_first + BK, k_last);
-    // (an odd count's last panel is followed by one of zeros)
-    for (int k0 = k_first; k0 <= k_last; k0 += 2 * BK) {
-      panel(ra[0], rb[0], k0, 0);
-      panel(ra[1], rb[1], k0 + BK, 1);
+#pragma unroll
+    for (int q = 0; q < S::AHEAD; ++q) a.load(ra[q], k_first + q * BK, k_last), b.load(rb[q], k_first + q * BK, k_last);
+    for (int k0 = k_first; k0 <= k_last; k0 += S::AHEAD * BK) {
+#pragma unroll
+      for (int q = 0; q < S::AHEAD; ++q) {
+        if (q > 0 && k0 + q * BK > k_last) break;
+        panel(ra[q], rb[q], k0 + q * BK, q & 1);
+      }
     }
     __syncthreads();
   }
