@@ -379,8 +379,26 @@ def test_wide_products_of_unaligned_operands(pkg, L, kind, ta, tb, M, N, K):
     check(gdb, db, edb, "dbias")
 
 
+@pytest.mark.parametrize("kind", ["f32", "f64"])
+@pytest.mark.parametrize("ta,tb", TRANS)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 70, 33), (65, 1, 16), (300, 200, 3), (605, 195, 174), (512, 8, 512), (3001, 17, 700), (64, 129, 2050)])
+def test_small_wide_products(pkg, L, kind, ta, tb, M, N, K):
+    """64 x 64 tiles: one element, one row, one column, less than a panel of k, whole panels and one more, K split."""
+    for lay in (Layout(), Layout(pad=1), Layout(pad=3, offset=1)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay)
+    opA, opB, Cm = rand_ints(M, K, 7), rand_ints(K, N, 8), rand_ints(M, N, 9, -9, 9)
+    got, _ = product(pkg, L, kind, ta, tb, opA, opB, alpha=2.0, beta=-1.0, Cm=Cm, in_place=True)
+    assert torch.equal(got, 2.0 * (opA @ opB) - Cm)
+    opA, opB, Z, Cm = rand(M, K, 31, kind, K ** -0.5), rand(K, N, 32, kind), rand(M, N, 33, kind, 2.0), rand(M, N, 34, kind)
+    for name in ("none", "relu", "gelu"):
+        d, ed, db, edb = gradient(opA, opB, Z, Cm, 1.0, 0.5, name, kind)
+        got, gdb = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, beta=0.5, Cm=Cm, name=name, lay=Layout(pad=1))
+        check(got, d, ed, "D")
+        check(gdb, db, edb, "dbias")
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("ta,tb,M,N,K", [("T", "N", 700, 300, 1001), ("N", "N", 256, 256, 4096), ("N", "T", 300, 200, 64), ("T", "T", 3, 5, 9), ("N", "N", 2051, 1701, 2003)])
+@pytest.mark.parametrize("ta,tb,M,N,K", [("T", "N", 700, 300, 1001), ("N", "N", 256, 256, 4096), ("N", "T", 300, 200, 64), ("T", "T", 3, 5, 9), ("N", "N", 2051, 1701, 2003), ("T", "N", 605, 195, 174), ("N", "N", 512, 8, 512)])
 def test_nothing_is_written_behind_the_workspace(pkg, L, kind, ta, tb, M, N, K):
     opA, opB, Z = rand_ints(M, K, 1), rand_ints(K, N, 2), rand_ints(M, N, 3)
     A, B = Mat(*((M, K) if ta == "N" else (K, M)), M if ta == "N" else K, kind).set(opA if ta == "N" else opA.T), Mat(*((K, N) if tb == "N" else (N, K)), K if tb == "N" else N, kind).set(opB if tb == "N" else opB.T)
