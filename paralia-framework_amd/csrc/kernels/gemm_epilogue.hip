@@ -2,7 +2,7 @@
 //   pl_gemm_epilogue        D = act(alpha * op(A) * op(B) + bias) + beta * C         (linear layer, weight gradient)
 //   pl_gemm_epilogue_grad   D = (alpha * op(A) * op(B) + beta * C) .* act'(Z), dbias (gradient through an activation)
 // 16-bit operands (bf16, fp16) run the kernels of half_product.h; fp32 and fp64 operands the library's tile GEMM
-// (gemm_mfma.hip) with the epilogue as one pass over its product.
+// (gemm_mfma.hip) with the epilogue as one pass over its product, small ones the kernel of wide_product.h.
 #include "kernels/epilogue.h"
 #include "kernels/linear.h"
 

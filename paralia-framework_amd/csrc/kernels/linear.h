@@ -135,8 +135,8 @@ inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
 // microseconds, fitted to 156 products of 64 x 64 x 64 to 8192 x 2048 x 2048: a 64 x 64 tile alone on its unit takes 0.053
 // (fp32 0.032) per k, several on one 0.039 (0.0245) each, and 2 (1) for its epilogue; a pass over slices 3, 0.8 for each slice
 // and their bytes at 4 TB/s.  The rule's choices are 2 % from the best of all measured ones, the tile GEMM's 26 %.
-// Both sides, fp64 / fp32, tile GEMM -> 64 x 64: 605 x 195 x 174 38 / 30 -> 17 / 11, 9472 x 192 x 3 21 / 17 -> 11 / 9,
-// 10474 x 17 x 2943 170 / 105 -> 99 / 69; 2048 x 2048 x 512 79 / 44 -> 87 / 54, 2048^3 256 / 133 -> 318 / 192.
+// Both sides, fp64 / fp32, tile GEMM -> 64 x 64: 605 x 195 x 174 38 / 30 -> 16 / 11, 9472 x 192 x 3 21 / 17 -> 11 / 8,
+// 10474 x 17 x 2943 170 / 105 -> 99 / 66; 2048 x 2048 x 512 79 / 44 -> 87 / 54, 2048^3 256 / 133 -> 318 / 192.
 struct WidePlan { int splits, kchunk; };
 inline WidePlan plan_wide(int es, bool at, bool bt, long M, long N, long K) {
   if (M > (1L << 27) || N > (1L << 27) || K > (1L << 30)) return {0, 0};
