@@ -30,14 +30,19 @@ def test_product_refuses(pkg, L, over, code):
     assert b"pl_gemm_epilogue:" in L.pl_last_error()
 
 
-def test_workspace_of_32_and_64_bit_products(pkg, L):
+@pytest.mark.parametrize("M,N,K", [(2048, 2048, 2048), (512, 8, 512)])
+def test_workspace_of_32_and_64_bit_products(pkg, L, M, N, K):
+    """A large product passes through the workspace, a long and narrow one in slices; a small one needs none."""
     for kind in (0, 1):
-        need = L.pl_gemm_epilogue_workspace_bytes(kind, b"T", b"N", 64, 32, 16, 0)
-        assert need >= 64 * 32 * (8 if kind == 0 else 4)
-        assert L.pl_gemm_epilogue_workspace_bytes(kind, b"T", b"N", 64, 32, 16, 1) > need
-        assert call(L, pkg, type=kind, ws=None, wsb=0) == 7
-        assert call(L, pkg, type=kind, ws=WS, wsb=need - 1) == 7
-        assert call(L, pkg, type=kind, ws=WS + 8, wsb=need) == 7
+        need = L.pl_gemm_epilogue_workspace_bytes(kind, b"T", b"N", M, N, K, 0)
+        assert need >= M * N * (8 if kind == 0 else 4)
+        assert L.pl_gemm_epilogue_workspace_bytes(kind, b"T", b"N", M, N, K, 1) > need
+        shape = dict(M=M, N=N, K=K, lda=K, ldb=K, ldd=M)
+        assert call(L, pkg, type=kind, ws=None, wsb=0, **shape) == 7
+        assert call(L, pkg, type=kind, ws=WS, wsb=need - 1, **shape) == 7
+        assert call(L, pkg, type=kind, ws=WS + 8, wsb=need, **shape) == 7
+        assert L.pl_gemm_epilogue_workspace_bytes(kind, b"T", b"N", 64, 32, 16, 0) == 0
+        assert L.pl_gemm_epilogue_workspace_bytes(kind, b"T", b"N", 64, 32, 16, 1) >= 64 * (8 if kind == 0 else 4)
     assert L.pl_gemm_epilogue_workspace_bytes(9, b"T", b"N", 64, 32, 16, 0) == 0
     assert L.pl_gemm_epilogue_workspace_bytes(3, b"T", b"N", 0, 32, 16, 1) == 0
 
