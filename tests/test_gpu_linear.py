@@ -347,6 +347,15 @@ def test_few_columns(pkg, L, kind, N, M, K):
     assert torch.equal(got, (2.0 * (opA @ opB) - Cm).to(TORCH[kind]).double())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(300, 9, 4103), (4263, 2, 1387), (130, 32, 2051), (600, 33, 1999)])
+def test_few_columns_of_unaligned_operands(pkg, L, kind, M, N, K):
+    """Odd strides and a ragged k: multiplied from copies whose k is filled up to whole panels."""
+    for lay in (Layout(), Layout(pad=1), Layout(pad=3, offset=5)):
+        exact_product(pkg, L, kind, "T", "N", M, N, K, lay)
+    exact_product(pkg, L, kind, "T", "N", M, N, K, Layout(pad=1), kind_d="f32", seed=4)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f64"])
 @pytest.mark.parametrize("ta,tb", TRANS)
 @pytest.mark.parametrize("M,N,K", [(256, 256, 4096), (1700, 1500, 1600), (700, 300, 1001)])
