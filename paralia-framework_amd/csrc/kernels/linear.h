@@ -132,9 +132,10 @@ inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
 
 // How an fp32 or fp64 product is launched: in the tile GEMM's tiles with the epilogue as a pass (splits 0), or in 64 x 64 tiles
 // with the epilogue inside, K split `splits` ways where it is long.  A function of the shape and the type alone.  Times in
-// microseconds, fitted to 156 products of 64 x 64 x 64 to 8192 x 2048 x 2048: a 64 x 64 tile alone on its unit takes 0.053
-// (fp32 0.032) per k, several on one 0.039 (0.0245) each, and 2 (1) for its epilogue; a pass over slices 3, 0.8 for each slice
-// and their bytes at 4 TB/s.  The rule's choices are 2 % from the best of all measured ones, the tile GEMM's 26 %.
+// microseconds, fitted to 216 products of 64 x 64 x 64 to 8192 x 2048 x 2048: a 64 x 64 tile alone on its unit takes 0.053
+// (fp32 0.032) per k, several on one 0.039 (0.0245) each, and 1 (0.5) for its epilogue; a pass over slices 3, and for each
+// slice 0.8 and its bytes at 5.7 TB/s (the memory-side cache holds them).  The rule's choices are 1 % from the best of all
+// measured ones, the tile GEMM's 24 %.
 // Both sides, fp64 / fp32, tile GEMM -> 64 x 64: 605 x 195 x 174 38 / 30 -> 16 / 11, 9472 x 192 x 3 21 / 17 -> 11 / 8,
 // 10474 x 17 x 2943 170 / 105 -> 99 / 66; 2048 x 2048 x 512 79 / 44 -> 87 / 54, 2048^3 256 / 133 -> 318 / 192.
 struct WidePlan { int splits, kchunk; };
@@ -153,15 +154,15 @@ inline WidePlan plan_wide(int es, bool at, bool bt, long M, long N, long K) {
       if ((k + kc - 1) / kc != s) continue;
     }
     const double per_unit = (double)((tiles * s + 255) / 256);
-    double us = 5.5 + (lone > per_unit * shared ? lone : per_unit * shared) * kc + per_unit * (0.25 * es) + 0.5 * cells_us;
-    if (s > 1) us += 3.0 + 0.8 * s + 2.0 * s * cells_us;
-    if (us < best_us * (s > 1 ? 0.95 : 1.0)) best_us = us, best = {s, s > 1 ? kc : 0};
+    double us = 5.5 + (lone > per_unit * shared ? lone : per_unit * shared) * kc + per_unit * (0.125 * es) + 0.5 * cells_us;
+    if (s > 1) us += 3.0 + (0.8 + 0.7 * cells_us) * s;
+    if (us < best_us) best_us = us, best = {s, s > 1 ? kc : 0};
   }
   if (best_us < 10.0 || K == 0) return best;   // (less than the tile GEMM's two launches ever take)
   const long per = 16 / es;
   const bool unaligned = (at ? K : M) % per != 0 || (bt ? N : K) % per != 0, ragged = M % 128 != 0 || N % 128 != 0 || K % 32 != 0;
   const double gemm = pl_gemm_tile_alone_us(es, at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, 1L << 28) * (unaligned ? (es == 4 ? 1.6 : 1.25) : ragged ? 1.1 : 1.0);
-  return best_us < 0.95 * (5.0 + gemm + 2.0 * cells_us) ? best : WidePlan{0, 0};
+  return best_us < 0.95 * (2.0 + gemm + 2.0 * cells_us) ? best : WidePlan{0, 0};
 }
 int wide_product_f32(const Call& c, const WidePlan& plan, bool at, bool bt, const Epilogue& ep, void* slices);
 int wide_product_f64(const Call& c, const WidePlan& plan, bool at, bool bt, const Epilogue& ep, void* slices);
