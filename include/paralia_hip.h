@@ -276,8 +276,9 @@ int pl_bias_act_grad(int type, int activation, long M, long N, const void* dY, l
 
 /* *norm <- sqrt of the sum of the squares of all elements of n tensors: tensor i has counts[i] elements of types[i] at
  * grads[i].  The three lists are host arrays that are free again when the call returns; the tensors, norm (one double) and
- * the workspace (pl_grad_norm_workspace_bytes(n) bytes, 16-byte aligned) are in device memory.  Squares are formed and
- * added in 64 bits, in an order that depends only on counts.  Infinities and NaN come through. */
+ * the workspace (pl_grad_norm_workspace_bytes(n) bytes, 16-byte aligned) are in device memory.  norm must lie outside the
+ * workspace.  Squares are formed and added in 64 bits, in an order that depends only on counts.  Infinities and NaN come
+ * through. */
 long pl_grad_norm_workspace_bytes(long n);
 int pl_grad_norm(long n, const void* const* grads, const long long* counts, const int* types, double* norm, void* workspace,
                  long workspace_bytes, void* stream);

@@ -266,6 +266,8 @@ int check_norm_args(const char* who, long n, const double* norm, const void* wor
   if (!norm) return refuse(PL_ERR_NULL, who, "null norm");
   if (!aligned_to(norm, 8)) return refuse(PL_ERR_ARG, who, "norm not 8-byte aligned");
   if (n > 0 && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < pl_grad_norm_workspace_bytes(n))) return refuse(PL_ERR_ARG, who, "workspace null, too small or not 16-byte aligned");
+  // the first workgroup of the scaling stores the norm while others still read the partial sums
+  if (n > 0 && overlap(bytes_at(norm, 8), bytes_at(workspace, pl_grad_norm_workspace_bytes(n)))) return refuse(PL_ERR_ARG, who, "norm overlaps the workspace");
   return PL_OK;
 }
 bool valid_limit(double max_norm, double eps) { return max_norm >= 0.0 && eps >= 0.0 && eps < 1e300; }

@@ -130,6 +130,20 @@ def test_workspaces_that_overlap_operands_are_refused(pkg, L):
         assert b"overlaps a tensor" in L.pl_last_error()
 
 
+def test_a_norm_inside_the_workspace_is_refused(L):
+    """The scaling reads the workspace's partial sums while its first workgroup stores the norm."""
+    need = L.pl_grad_norm_workspace_bytes(2)
+    ptrs, counts, types = (C.c_void_p * 2)(A, B), (C.c_longlong * 2)(100, 200), (C.c_int * 2)(1, 3)
+    for norm in (WS, WS + 8, WS + need - 8):
+        assert clip(L, [A, B], [100, 200], [1, 3], [A, B], norm=norm) == 7, hex(norm)
+        assert b"pl_grad_norm_clip: norm overlaps the workspace" in L.pl_last_error()
+        assert L.pl_grad_norm(2, ptrs, counts, types, norm, WS, need, None) == 7, hex(norm)
+        assert b"pl_grad_norm: norm overlaps the workspace" in L.pl_last_error()
+    # right behind the bytes that a call uses it is taken: the next check answers
+    assert clip(L, [A, B], [100, 200], [1, 3], [A, B], norm=WS + need, max_norm=-1.0) == 7
+    assert b"max_norm" in L.pl_last_error()
+
+
 def test_rows_beyond_the_fold(L):
     assert act_grad(L, M=(1 << 27) + 1, N=1, lddy=1 << 28, ldz=1 << 28, lddz=1 << 28) == 2
     assert grad(L, M=(1 << 27) + 1, N=1, K=1, lda=1 << 28, ldz=1 << 28, ldd=1 << 28) == 2
