@@ -13,9 +13,9 @@ namespace plk {
 constexpr int PASS_THREADS = 256;
 
 // v(m, n) <- sum over slices of P(m, n), through the epilogue.  blockIdx.x: 64 * VEC rows, blockIdx.y: a range of `per`
-// columns.  GRAD with ep.partial: row blockIdx.y of the partial sums.
+// columns.  GRAD with ep.partial: row blockIdx.y of the partial sums.  (P is not __restrict__: it may be D, as C and Z may.)
 template <typename TP, typename T, typename TD, bool GRAD, bool SLICES, int VEC>
-__global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, long N, long per, const TP* __restrict__ P, long ldP, long slice, int slices,
+__global__ __launch_bounds__(PASS_THREADS) void epilogue_pass_kernel(long M, long N, long per, const TP* P, long ldP, long slice, int slices,
                                                                     Epilogue ep) {
   using W = wide_t<T>;
   __shared__ W fold[GRAD ? 4 * 64 * VEC : 1];

@@ -288,11 +288,13 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN * STAGES <= 128 * 128 * 2 ? 2 :
     // last step: from there on every wave has read all of panel kt, panel kt + 1 is complete, and the requests of panel
     // kt + STAGES may fill panel kt's buffer, the first half of them at once, the rest during the next panel's first step.
     // The source is in issue order, an MFMA and then what goes out behind it.  STEADY: all those panels exist.
-    // (__restrict__: a transposing read that the compiler cannot tell from the requests' buffer waits for all of them.)
+    // (__restrict__: a transposing read that the compiler cannot tell from the requests' buffer waits for all of them.  With two
+    // stages the buffer behind this panel's is also the one before it: it is then reached through nxt alone.)
     const short* next_a = Ab + (STAGES - 1) * a_step;   // the panel that is being asked for
     const short* next_b = Bb + (STAGES - 1) * b_step;
     constexpr int NEWER = (STAGES - 2) * NR;   // requests that may be out when panel kt + 1 has landed
     auto panel = [&]<bool STEADY>(int kt, short* __restrict__ cur, short* __restrict__ nxt, short* __restrict__ prv) __attribute__((always_inline)) {
+      short* const fill = STAGES == 2 ? nxt : prv;
       const bool ask1 = STEADY || kt + STAGES - 1 < nfull, ask2 = STEADY || kt + STAGES < nfull, next = STEADY || kt + 1 < nfull;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(H_THREADS, (BM * BN * STAGES <= 128 * 128 * 2 ? 2 :
           if (s == 0 && ask1) {
 #pragma unroll
             for (int r = EARLY; r < NR; ++r)
-              if ((r - EARLY) * MFMAS / (NR - EARLY) == m) ask(pa, pb, prv, r);
+              if ((r - EARLY) * MFMAS / (NR - EARLY) == m) ask(pa, pb, fill, r);
           }
           if (last && ask2) {
 #pragma unroll
