@@ -30,9 +30,9 @@ inline Workspace workspace_for(int type, const HalfPlan& p, const WidePlan& wp, 
     // the slices of a product alone on the device, or the product and behind it the slices of its tail; of the operands and
     // of their copies, whichever the call will be given
     const char ta = at ? 'T' : 'N', tb = bt ? 'T' : 'N';
-    long slices = pl_gemm_tile_alone_workspace_bytes(ta, tb, M, N, K, 1, (int)wide);
+    long slices = product_alone_slices_bytes((int)wide, ta, tb, M, N, K);
     if (copies.bytes() > 0) {
-      const long padded = pl_gemm_tile_alone_workspace_bytes(ta, tb, M, N, whole(K, WIDE_K), 1, (int)wide);
+      const long padded = product_alone_slices_bytes((int)wide, ta, tb, M, N, whole(K, WIDE_K));
       if (padded > slices) slices = padded;
     }
     w.product = round16(M * N * wide) + round16(slices);
@@ -167,8 +167,8 @@ int run_product(Call& c) {
     const bool f64 = c.type == PL_TYPE_F64;
     if (plain_product(c)) {
       // nothing but the product (and C where D is): the tile GEMM's own epilogue
-      return f64 ? pl_dgemm_tile_padded(c.ta, c.tb, M, N, c.K, ep.alpha, (const double*)c.A, c.lda, (const double*)c.B, c.ldb, ep.beta, (double*)ep.D, ep.ldd, ws, w.product, -1, m_read, n_read, c.stream)
-                 : pl_sgemm_tile_padded(c.ta, c.tb, M, N, c.K, (float)ep.alpha, (const float*)c.A, c.lda, (const float*)c.B, c.ldb, (float)ep.beta, (float*)ep.D, ep.ldd, ws, w.product, -1, m_read, n_read, c.stream);
+      return f64 ? product_alone_f64(c.ta, c.tb, M, N, c.K, ep.alpha, c.A, c.lda, c.B, c.ldb, ep.beta, ep.D, ep.ldd, ws, w.product, m_read, n_read, c.stream)
+                 : product_alone_f32(c.ta, c.tb, M, N, c.K, (float)ep.alpha, c.A, c.lda, c.B, c.ldb, (float)ep.beta, ep.D, ep.ldd, ws, w.product, m_read, n_read, c.stream);
     }
     int slices = 1;
     rc_ = (f64 ? product_slices_f64 : product_slices_f32)(c.ta, c.tb, M, N, c.K, c.A, c.lda, c.B, c.ldb, ws, w.product, m_read, n_read, f64 && c.grad, &slices, c.stream);

@@ -921,6 +921,13 @@ inline pl_gemm_fit& fit_in_use() {
   static pl_gemm_fit f = [] { pl_gemm_fit d; fit_defaults(&d); return d; }();
   return f;
 }
+// The built-in values, for callers whose choices may depend on the shape alone (the linear layers: their workspace is sized
+// once, and their sums keep their order).  Below, a `fixed` fit stands for that: these constants, and no pins out of the
+// environment; null is the routines' own rule.
+const pl_gemm_fit& fit_builtin() {
+  static const pl_gemm_fit f = [] { pl_gemm_fit d; fit_defaults(&d); return d; }();
+  return f;
+}
 
 template <typename T>
 int pick_splits(long M, long N, long K, int* kchunk_out) {
@@ -964,10 +971,10 @@ int pick_splits(long M, long N, long K, int* kchunk_out) {
 // and the reduction's pass over the slices and C (the slices' way out of the workgroups is part of their epilogue, as the
 // write of C is).  *us_out: the predicted time of the choice.
 template <typename T>
-int pick_splits_alone(long M, long N, long K, long max_ws_bytes, int* kchunk_out, double* us_out) {
+int pick_splits_alone(long M, long N, long K, long max_ws_bytes, int* kchunk_out, double* us_out, const pl_gemm_fit* fixed) {
   constexpr int BM = 128, BN = 128;
   const long tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  const pl_gemm_fit& fit = fit_in_use();
+  const pl_gemm_fit& fit = fixed ? *fixed : fit_in_use();
   const double c1 = fit.lone_us_per_k[sizeof(T) == 8 ? 0 : 1];
   const double c2 = c1 * fit.f32_small_us_per_k / fit.lone_us_per_k[1];
   const double f = fit.lone_fixed_k * c1;
@@ -1005,12 +1012,12 @@ int pick_splits_alone(long M, long N, long K, long max_ws_bytes, int* kchunk_out
 // the terms of pick_splits_alone plus half a split's launch cost for the extra launch; taken when 3 % ahead of
 // best_us, the best of the one-launch choices.  Returns the tail's split count (0: one launch stays).
 template <typename T>
-int pick_tail_alone(long M, long N, long K, long max_ws_bytes, double best_us, long* n_head_out, double* us_out) {
+int pick_tail_alone(long M, long N, long K, long max_ws_bytes, double best_us, long* n_head_out, double* us_out, const pl_gemm_fit* fixed) {
   constexpr int BM = 128, BN = 128;
   const long gm = (M + BM - 1) / BM, gn = (N + BN - 1) / BN;
-  const char* const off = getenv("PARALIA_GEMM_TAIL");
+  const char* const off = fixed ? nullptr : getenv("PARALIA_GEMM_TAIL");
   if ((off && *off == '0') || gn < 2 || K < 512 || gm * gn <= 512) return 0;
-  const pl_gemm_fit& fit = fit_in_use();
+  const pl_gemm_fit& fit = fixed ? *fixed : fit_in_use();
   const double c1 = fit.lone_us_per_k[sizeof(T) == 8 ? 0 : 1];
   const double c2 = c1 * fit.f32_small_us_per_k / fit.lone_us_per_k[1];
   const double f = fit.lone_fixed_k * c1;
@@ -1054,7 +1061,7 @@ int pick_tail_alone(long M, long N, long K, long max_ws_bytes, double best_us, l
 struct TileChoice { int tm = 128, tn = 128, splits = 1, kchunk = 0; bool big = false, wide = false; long n_head = 0; int tail_splits = 0; double us = -1; };
 template <typename T>
 TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero, bool have_ws, long workspace_bytes, bool large_allowed = true,
-                       int want_splits = 0, bool alone = false, long m_read = 0, long n_read = 0, bool small_only = false) {
+                       int want_splits = 0, bool alone = false, long m_read = 0, long n_read = 0, bool small_only = false, const pl_gemm_fit* fixed = nullptr) {
   TileChoice c;
   double alone_us = -1;   // alone: the predicted time of the 128 x 128 tile with the split count chosen for it
   if (want_splits >= 1) {
@@ -1064,7 +1071,7 @@ TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero
     const long se = (K + kc - 1) / kc;
     if (se > 1 && have_ws && want_splits > 1) c.splits = (int)se, c.kchunk = (int)kc;
   } else if (alone) {
-    c.splits = pick_splits_alone<T>(M, N, K, have_ws ? workspace_bytes : 0, &c.kchunk, &alone_us);
+    c.splits = pick_splits_alone<T>(M, N, K, have_ws ? workspace_bytes : 0, &c.kchunk, &alone_us, fixed);
   } else {
     c.splits = have_ws ? pick_splits<T>(M, N, K, &c.kchunk) : 1;
   }
@@ -1084,7 +1091,7 @@ TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero
   // The constants are pl_gemm_fit's (built-in: c = 0.1099 us, f_s = 7.4 us, f_w = 4.9 | 10.6 us, g = 0.010 - 0.012, f = 11 |
   // 45 - 54 us).  Split K keeps the small tile.  fp64 stays at 128 x 128: a 256 x 128 tile (one wave per SIMD,
   // 32-cycle MFMAs) measured 70.7 against 73.4 TFLOP/s.
-  const pl_gemm_fit& fit = fit_in_use();
+  const pl_gemm_fit& fit = fixed ? *fixed : fit_in_use();
   const int tr = an ? (bnn ? 0 : 1) : (bnn ? 2 : 3);
   const int bi = beta_zero ? 0 : 1;
   auto tiles_of = [&](long tm, long tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
@@ -1109,7 +1116,7 @@ TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero
   int cut_splits = 0;
   if (alone_us >= 0 && have_ws) {
     double cut_us = -1;
-    cut_splits = pick_tail_alone<T>(M, N, K, workspace_bytes, alone_us, &cut_head, &cut_us);
+    cut_splits = pick_tail_alone<T>(M, N, K, workspace_bytes, alone_us, &cut_head, &cut_us, fixed);
     if (cut_splits > 1) alone_us = cut_us;
   }
   if (alone_us >= 0) alone_us += small_edge_us;
@@ -1118,7 +1125,7 @@ TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero
   const double wide_us = (double)((tiles_of(256, 128) + 511) / 512) * wide_round + (edge(256, 128) ? fit.edge_rounds[0] * wide_round : 0.0);
   // PARALIA_GEMM_LARGE_TILE: "0" small tiles only, "1" the large tile for every call, "2" the wide tile wherever it
   // exists (NN), unset: the model
-  const char* const pin = getenv("PARALIA_GEMM_LARGE_TILE");
+  const char* const pin = fixed ? nullptr : getenv("PARALIA_GEMM_LARGE_TILE");
   const int pinv = (pin && *pin) ? atoi(pin) : -1;
   // (alone, the bigger tiles are weighed against the split small tile too; a caller's own split count keeps the small one)
   const bool other = sizeof(T) == 4 && (c.splits == 1 || alone_us >= 0) && pinv != 0 && !small_only;
@@ -1140,7 +1147,8 @@ TileChoice choose_tile(bool an, bool bnn, long M, long N, long K, bool beta_zero
 template <typename T>
 int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, long lda, const T* B, long ldb, T beta,
                 T* C, long ldc, hipStream_t stream, T* workspace = nullptr, long workspace_bytes = 0, int want_splits = 0,
-                bool alone = false, long m_read = 0, long n_read = 0, bool small_only = false, bool leave_slices = false) {
+                bool alone = false, long m_read = 0, long n_read = 0, bool small_only = false, bool leave_slices = false,
+                const pl_gemm_fit* fixed = nullptr) {
   using Tr = Traits<T>;
   const bool at = (ta == 'T' || ta == 't'), an = (ta == 'N' || ta == 'n');
   const bool bt = (tb == 'T' || tb == 't'), bnn = (tb == 'N' || tb == 'n');
@@ -1165,15 +1173,15 @@ int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, l
   // a K-major operand loaded straight into LDS takes eight rows per request with 32-bit lane offsets: leading dimensions
   // beyond that keep the tiles that stage through registers
   const bool dma_fits = (!at || lda * (long)sizeof(T) <= PLK_DMA_MAX_LD_BYTES) && (!bnn || ldb * (long)sizeof(T) <= PLK_DMA_MAX_LD_BYTES);
-  const TileChoice choice = choose_tile<T>(an, bnn, M, N, K, beta == T(0), workspace != nullptr, workspace_bytes, dma_fits, want_splits, alone, m_read, n_read, small_only);
+  const TileChoice choice = choose_tile<T>(an, bnn, M, N, K, beta == T(0), workspace != nullptr, workspace_bytes, dma_fits, want_splits, alone, m_read, n_read, small_only, fixed);
   if (choice.tail_splits > 1) {
     // head: whole tile columns, unsplit, in the 128 x 128 tiles the cut was priced with; tail: the remaining columns of
     // op(B) and C with K split
     const long nh = choice.n_head;
-    const int rc = launch_gemm<T>(ta, tb, M, nh, K, alpha, A, lda, B, ldb, beta, C, ldc, stream, nullptr, 0, 1, false, m_read, n_read, true);
+    const int rc = launch_gemm<T>(ta, tb, M, nh, K, alpha, A, lda, B, ldb, beta, C, ldc, stream, nullptr, 0, 1, false, m_read, n_read, true, false, fixed);
     if (rc != 0) return rc;
     return launch_gemm<T>(ta, tb, M, N - nh, K, alpha, A, lda, bnn ? B + nh * ldb : B + nh, ldb, beta, C + nh * ldc, ldc, stream, workspace,
-                          workspace_bytes, choice.tail_splits, false, m_read, n_read - nh);
+                          workspace_bytes, choice.tail_splits, false, m_read, n_read - nh, false, false, fixed);
   }
   const int kchunk = choice.kchunk, splits = choice.splits;
   const bool big = choice.big, wide = choice.wide;
@@ -1229,18 +1237,49 @@ int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, l
   return hipGetLastError() == hipSuccess ? 0 : 4;
 }
 
+// workspace a product alone on the device is given at most (the slices of its split)
+#define PLK_ALONE_MAX_WS_BYTES (1L << 30)
+
+// What the linear layers' launcher asks and calls, under the built-in fit.
+// A product alone on the device, beta == 0: its predicted time with a workspace of ws_bytes, and the slices it needs.
+template <typename T>
+TileChoice fixed_choice(char ta, char tb, long M, long N, long K, long ws_bytes) {
+  const bool an = ta == 'N' || ta == 'n', bnn = tb == 'N' || tb == 'n';
+  return choose_tile<T>(an, bnn, M, N, K, true, ws_bytes > 0, ws_bytes, true, 0, true, 0, 0, false, &fit_builtin());
+}
+double product_alone_us(int elem_size, char ta, char tb, long M, long N, long K, long ws_bytes) {
+  return elem_size == 8 ? fixed_choice<double>(ta, tb, M, N, K, ws_bytes).us : fixed_choice<float>(ta, tb, M, N, K, ws_bytes).us;
+}
+long product_alone_slices_bytes(int elem_size, char ta, char tb, long M, long N, long K) {
+  if (K <= 0) return 0;
+  const TileChoice c = elem_size == 8 ? fixed_choice<double>(ta, tb, M, N, K, PLK_ALONE_MAX_WS_BYTES) : fixed_choice<float>(ta, tb, M, N, K, PLK_ALONE_MAX_WS_BYTES);
+  if (c.tail_splits > 1) return (long)c.tail_splits * M * (N - c.n_head) * elem_size;
+  return c.splits > 1 ? (long)c.splits * M * N * elem_size : 0;
+}
+// The product with nothing behind it but beta * C where D is C.
+int product_alone_f32(char ta, char tb, long M, long N, long K, float alpha, const void* A, long lda, const void* B, long ldb, float beta, void* C, long ldc, void* ws,
+                      long ws_bytes, long m_read, long n_read, hipStream_t stream) {
+  return launch_gemm<float>(ta, tb, M, N, K, alpha, (const float*)A, lda, (const float*)B, ldb, beta, (float*)C, ldc, stream, (float*)ws, ws_bytes, 0, true, m_read, n_read,
+                            false, false, &fit_builtin());
+}
+int product_alone_f64(char ta, char tb, long M, long N, long K, double alpha, const void* A, long lda, const void* B, long ldb, double beta, void* C, long ldc, void* ws,
+                      long ws_bytes, long m_read, long n_read, hipStream_t stream) {
+  return launch_gemm<double>(ta, tb, M, N, K, alpha, (const double*)A, lda, (const double*)B, ldb, beta, (double*)C, ldc, stream, (double*)ws, ws_bytes, 0, true, m_read,
+                             n_read, false, false, &fit_builtin());
+}
 // For a caller that finishes the product itself (the fused epilogue of the linear layers): op(A) * op(B) as a product alone
 // on the device would run it, into `slices` dense M x N slices at ws that are still to be added (1, or add: the product itself).
 template <typename T>
 int product_slices(char ta, char tb, long M, long N, long K, const T* A, long lda, const T* B, long ldb, T* ws, long ws_bytes, long m_read, long n_read,
                    bool add, int* slices, hipStream_t stream) {
   const bool an = ta == 'N' || ta == 'n', bnn = tb == 'N' || tb == 'n';
-  *slices = K > 0 ? choose_tile<T>(an, bnn, M, N, K, true, true, ws_bytes, true, 0, true, m_read, n_read).splits : 1;
+  *slices = K > 0 ? choose_tile<T>(an, bnn, M, N, K, true, true, ws_bytes, true, 0, true, m_read, n_read, false, &fit_builtin()).splits : 1;
   if (add) *slices = 1;
-  if (*slices > 1) return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, ws, ws_bytes, *slices, false, m_read, n_read, false, true);
+  if (*slices > 1) return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, ws, ws_bytes, *slices, false, m_read, n_read, false, true, &fit_builtin());
   // one launch, or an unsplit head and a split tail whose slices lie behind the product
   const long product = (M * N * (long)sizeof(T) + 15) & ~15L;
-  return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, (T*)((char*)ws + product), ws_bytes - product, 0, true, m_read, n_read);
+  return launch_gemm<T>(ta, tb, M, N, K, T(1), A, lda, B, ldb, T(0), ws, M, stream, (T*)((char*)ws + product), ws_bytes - product, 0, true, m_read, n_read, false,
+                        false, &fit_builtin());
 }
 int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
                        int* slices, hipStream_t stream) {
@@ -1340,9 +1379,6 @@ extern "C" int pl_sgemm_tile_padded(char transA, char transB, long M, long N, lo
   return plk::launch_gemm<float>(transA, transB, M, N, K, alpha, A, lda, B, ldb, beta, C, ldc, (hipStream_t)stream,
                                  (float*)workspace, workspace_bytes, splits < 0 ? 0 : splits, splits < 0, m_readable, n_readable);
 }
-
-// workspace a product alone on the device is given at most (the slices of its split)
-#define PLK_ALONE_MAX_WS_BYTES (1L << 30)
 
 extern "C" int pl_dgemm_tile_alone(char transA, char transB, long M, long N, long K, double alpha, const double* A, long lda,
                                    const double* B, long ldb, double beta, double* C, long ldc, void* workspace,

@@ -60,7 +60,16 @@ inline bool same_or_apart(const Range& a, const Range& b) {
   return (a.p == b.p && (a.ld == b.ld || a.cols == 1) && a.size == b.size) || !overlap(a, b);
 }
 
-// gemm_mfma.hip: the fp32 / fp64 product in slices that are still to be added
+// gemm_mfma.hip: the fp32 / fp64 product alone on the device, all under the tile GEMM's built-in constants, so that neither a
+// database that is loaded later nor the environment changes a plan.  Its predicted time and the slices it needs,
+double product_alone_us(int elem_size, char ta, char tb, long M, long N, long K, long ws_bytes);
+long product_alone_slices_bytes(int elem_size, char ta, char tb, long M, long N, long K);
+// the product itself,
+int product_alone_f32(char ta, char tb, long M, long N, long K, float alpha, const void* A, long lda, const void* B, long ldb, float beta, void* C, long ldc, void* ws,
+                      long ws_bytes, long m_read, long n_read, hipStream_t stream);
+int product_alone_f64(char ta, char tb, long M, long N, long K, double alpha, const void* A, long lda, const void* B, long ldb, double beta, void* C, long ldc, void* ws,
+                      long ws_bytes, long m_read, long n_read, hipStream_t stream);
+// or its slices that are still to be added.
 int product_slices_f32(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
                        int* slices, hipStream_t stream);
 int product_slices_f64(char ta, char tb, long M, long N, long K, const void* A, long lda, const void* B, long ldb, void* ws, long ws_bytes, long m_read, long n_read, bool add,
@@ -161,7 +170,7 @@ inline WidePlan plan_wide(int es, bool at, bool bt, long M, long N, long K) {
   if (best_us < 10.0 || K == 0) return best;   // (less than the tile GEMM's two launches ever take)
   const long per = 16 / es;
   const bool unaligned = (at ? K : M) % per != 0 || (bt ? N : K) % per != 0, ragged = M % 128 != 0 || N % 128 != 0 || K % 32 != 0;
-  const double gemm = pl_gemm_tile_alone_us(es, at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1, 1L << 28) * (unaligned ? (es == 4 ? 1.6 : 1.25) : ragged ? 1.1 : 1.0);
+  const double gemm = product_alone_us(es, at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1L << 28) * (unaligned ? (es == 4 ? 1.6 : 1.25) : ragged ? 1.1 : 1.0);
   return best_us < 0.95 * (2.0 + gemm + 2.0 * cells_us) ? best : WidePlan{0, 0};
 }
 int wide_product_f32(const Call& c, const WidePlan& plan, bool at, bool bt, const Epilogue& ep, void* slices);

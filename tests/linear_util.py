@@ -4,7 +4,9 @@ that 32-bit (64-bit) arithmetic may leave.
 Notation of the bounds: u = 2^-24 (2^-53 for fp64 operands), S = |alpha| |A| |B| + |bias| with the operands' magnitudes.
 A product summed in any order, with the accumulator rounded (or truncated) after every step, is off by at most
 2 (K + 2) u S.  An activation's slope is below 1.13, so that error grows by at most that much on its way through it."""
+import ctypes as C
 import math
+import os
 
 import torch
 
@@ -133,3 +135,28 @@ def check(got, want, bound, what):
     assert not bool(bad.any()), "%s: %d of %d elements off, worst %.3g of the bound, first at %s: %r instead of %r" % (
         what, int(bad.sum()), bad.numel(), float((off / bound).nan_to_num(nan=float("inf")).max()), bad.nonzero()[0].tolist(),
         float(got[bad][0]), float(want[bad][0]))
+
+
+def shipped_fit(pkg, L):
+    """The launcher constants of the shipped database, as the library's first routine call installs them."""
+    import sys
+    f = sys.modules[pkg.__name__ + ".binding"].gemm_fit()
+    L.pl_gemm_fit_defaults(C.byref(f))
+    names = {"lone_us_per_k_f64": ("lone_us_per_k", 0), "lone_us_per_k_f32": ("lone_us_per_k", 1), "f32_wide_fixed_us_beta0": ("f32_wide_fixed_us", 0),
+             "f32_wide_fixed_us_beta1": ("f32_wide_fixed_us", 1), "edge_rounds_small": ("edge_rounds", 0), "edge_rounds_large": ("edge_rounds", 1)}
+    for t, trans in enumerate(("NN", "NT", "TN", "TT")):
+        names["f32_large_gain_" + trans] = ("f32_large_gain", t)
+        for b in range(2):
+            names["f32_large_fixed_us_beta%d_%s" % (b, trans)] = ("f32_large_fixed_us", t, b)
+    fields = {name for name, _ in f._fields_}
+    for line in open(os.path.join(pkg.PKG_DIR, "db", "mi355x", "Processed", "Kernel-fit_dev-0.log")):
+        name, _, value = line.partition(":")
+        if name in names:
+            field, at = names[name][0], names[name][1:]
+            array = getattr(f, field)
+            for i in at[:-1]:
+                array = array[i]
+            array[at[-1]] = float(value)
+        elif name in fields:
+            setattr(f, name, float(value))
+    return f

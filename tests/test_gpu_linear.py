@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from linear_util import ACTS, TORCH, TYPES, Mat, check, forward, gradient, half_step, slope_product
+from linear_util import ACTS, TORCH, TYPES, Mat, check, forward, gradient, half_step, shipped_fit, slope_product
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -300,6 +300,23 @@ def test_results_repeat_bit_for_bit(pkg, L):
     for _ in range(3):
         again = product_grad(pkg, L, "bf16", "N", "N", opA, opB, Z, name="gelu")
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("kind,ta,tb,M,N,K", [("f64", "T", "N", 128, 1216, 5824), ("f32", "T", "N", 256, 6848, 1024), ("f32", "N", "T", 2560, 400, 384), ("f64", "N", "T", 5516, 74, 2205)])
+def test_results_do_not_depend_on_the_routines_constants(pkg, L, kind, ta, tb, M, N, K):
+    """The same bits before and after a routine has installed the database's launcher constants, in the workspace asked for
+    before."""
+    opA, opB, Z = rand(M, K, 1, kind, K ** -0.5), rand(K, N, 2, kind), rand(M, N, 3, kind)
+    first, plain = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="silu"), product(pkg, L, kind, ta, tb, opA, opB)
+    need = [L.pl_gemm_epilogue_workspace_bytes(TYPES[kind], ta.encode(), tb.encode(), M, N, K, db) for db in (0, 1)]
+    try:
+        assert L.pl_gemm_set_fit(C.byref(shipped_fit(pkg, L))) == 0
+        assert need == [L.pl_gemm_epilogue_workspace_bytes(TYPES[kind], ta.encode(), tb.encode(), M, N, K, db) for db in (0, 1)]
+        again = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="silu")
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+        assert torch.equal(plain[0], product(pkg, L, kind, ta, tb, opA, opB)[0])
+    finally:
+        assert L.pl_gemm_set_fit(None) == 0
 
 
 # ---- the launcher's other ways: large tiles, split K, few columns, copies of unaligned operands ----

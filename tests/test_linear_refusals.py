@@ -1,8 +1,11 @@
 """What the linear-layer operators and the gradient norm refuse, on the host and before anything is launched: no device
 is needed to see the status codes, and pl_last_error() names the entry point."""
 import ctypes as C
+import random
 
 import pytest
+
+from linear_util import shipped_fit
 
 A, B, CM, D, Z, DB, WS = (0x10000000 * i for i in range(1, 8))   # addresses nobody dereferences
 
@@ -154,3 +157,31 @@ def test_nothing_to_do_is_no_error(pkg, L):
     assert call(L, pkg, N=0) == 0
     assert act_grad(L, M=0) == 0
     assert act_grad(L, N=0, db=None) == 0
+
+
+def test_the_workspace_is_a_function_of_the_shape_alone(pkg, L, monkeypatch):
+    """What a program asked for at its start is enough after a routine has installed the database's launcher constants, and
+    whatever the environment pins for the routines' own products."""
+    rng = random.Random(7)
+    shapes = [(0, b"T", b"N", 128, 1216, 5824), (1, b"T", b"N", 256, 6848, 1024), (1, b"N", b"T", 2560, 400, 384), (0, b"N", b"T", 5516, 74, 2205)]
+    for _ in range(4000):
+        shapes.append((rng.choice([0, 1]), rng.choice([b"N", b"T"]), rng.choice([b"N", b"T"]), *(int(round(2 ** rng.uniform(3, 13))) for _ in range(3))))
+    ask = lambda: [L.pl_gemm_epilogue_workspace_bytes(*s, db) for s in shapes for db in (0, 1)]  # noqa: E731
+    before = ask()
+    try:
+        assert L.pl_gemm_set_fit(C.byref(shipped_fit(pkg, L))) == 0
+        assert ask() == before
+        for s, need in list(zip(shapes, before[::2]))[:4]:
+            if need == 0:
+                continue
+            kind, ta, tb, M, N, K = s
+            # (an operand inside the workspace, so that the check behind its size answers, and nothing is launched)
+            over = dict(type=kind, ta=ta, tb=tb, M=M, N=N, K=K, lda=max(M, K), ldb=max(N, K), ldd=M, A=WS, ws=WS, wsb=need, D=WS * 16)
+            assert call(L, pkg, **over) == 7
+            assert b"overlaps an operand" in L.pl_last_error()
+    finally:
+        assert L.pl_gemm_set_fit(None) == 0
+    for name, value in (("PARALIA_GEMM_TAIL", "0"), ("PARALIA_GEMM_LARGE_TILE", "0"), ("PARALIA_GEMM_LARGE_TILE", "1"), ("PARALIA_GEMM_LARGE_TILE", "2")):
+        with monkeypatch.context() as m:
+            m.setenv(name, value)
+            assert ask() == before, (name, value)
