@@ -163,3 +163,26 @@ def test_repeats_bit_for_bit(pkg, L):
     for _ in range(3):
         assert clip(pkg, L, t, 1.0, False) == first
         assert all(torch.equal(a, b) for a, b in zip(outs, t.out_views))
+
+
+def whole_lists(n, seed, biggest):
+    """n tensors, none of them empty."""
+    return [(count + 1, kind, offset) for count, kind, offset in mixed(n, seed, biggest)]
+
+
+@pytest.mark.parametrize("n", [127, 128, 129, 255, 256, 257])
+def test_lists_around_a_launch(pkg, L, n):
+    """128 tensors go into a launch: one fewer, as many, one more, and the same around the second; bounds as above."""
+    for in_place, factor in ((False, 0.25), (True, 0.25), (True, 4.0)):
+        t = Tensors(whole_lists(n, n, 300), 5)
+        before = [v.double().clone() for v in t.views]
+        total = sum(v.numel() for v in t.views)
+        norm = t.norm()
+        got = clip(pkg, L, t, factor * norm, in_place)
+        assert abs(got - norm) <= norm * (total + 4) * 2.0 ** -53
+        scale = min(1.0, factor * norm / (norm + EPS))
+        for v, o, b, kind in zip(t.views, t.out_views, before, t.kinds):
+            u = 2.0 ** -52 if kind == "f64" else 2.0 ** -23
+            err = (b * scale).abs() * (u * 2 + (total + 4) * 2.0 ** -52) if scale < 1.0 else torch.zeros_like(b)
+            out = (v if in_place else o).double()
+            assert bool(((out - b * scale).abs() <= err + (half_step((b * scale).abs() + err, kind) if scale < 1.0 else 0.0)).all())
