@@ -3,9 +3,9 @@
 //
 // HBM bounds both passes: the norm reads every element once, the scaling reads and writes it once.  The tensors are cut
 // into chunks of CHUNK elements that never span two tensors, and a fixed number of workgroups walks all chunks of up to
-// LIST_MAX tensors in one launch, so that thousands of small tensors cost a few launches and a large one is spread over
-// the chip.  Pointers and counts travel in the kernel's arguments: no table in device memory to keep, to copy or to go
-// stale, and a captured launch holds its own.
+// LIST_MAX tensors in one launch, so that many small tensors cost two launches for each 128 of them and a large one is
+// spread over the chip.  Pointers and counts travel in the kernel's arguments: no table in device memory to keep, to copy
+// or to go stale, and a captured launch holds its own.
 //
 // Squares are formed and added in 64 bits (a 32-bit square of a 32-bit gradient below 1e-23 or above 1e19 is lost; the
 // conversion and the 64-bit fma run at several times the rate at which memory delivers elements).  The order of the sum
@@ -111,6 +111,7 @@ __global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(TensorList l
 
 __device__ __forceinline__ double fold_norm(const double* __restrict__ partial, int partials) {
   double s = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < partials; i += NORM_THREADS) s += partial[i];
   return sqrt(sum_block(s));
 }
@@ -136,8 +137,11 @@ template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T*
   }
 }
 
-// partials > 0: every workgroup folds the partial sums of the norm's launches itself, in the same order (16 KiB out of the
-// L2 against a launch of its own), and workgroup 0 of the first launch stores the norm.  partials == 0: *norm is given.
+// partials > 0: every workgroup folds the partial sums of the norm's launches itself, in the same order (at most 16 KiB out
+// of the L2, against a launch of its own), and workgroup 0 of the first launch stores the norm.  partials == 0: *norm is
+// given, or folded already: with more partial sums than one launch leaves, every workgroup of every launch would read all
+// of them again, work that grows with the square of the list (bf16 tensors of
+// 100 k elements, folded everywhere / once: 1000 of them 240 / 162 us, 5000 2719 / 858; 300 of 70 k 52 / 51).
 // A factor of exactly 1 leaves tensors that are scaled in place as they are.
 __global__ __launch_bounds__(NORM_THREADS) void grad_scale_kernel(TensorList list, const double* __restrict__ partial, int partials, int store, double max_norm,
                                                                  double eps, double* norm) {
@@ -337,6 +341,11 @@ extern "C" int pl_grad_norm_clip(long n, const void* const* grads, const long lo
     rc = launch_squares(n, grads, counts, types, (double*)workspace, &partials, s);
     if (rc != PL_OK) return rc;
     if (partials == 0) return grad_norm_only(0, grads, counts, types, norm, (double*)workspace, s);   // nothing to scale: a norm of zero
+    if (partials > NORM_BLOCKS) {
+      rc = launch(grad_norm_kernel, dim3(1), dim3(NORM_THREADS), s, (const double*)workspace, partials, norm);
+      if (rc != PL_OK) return rc;
+      partials = 0;
+    }
     return launch_scale(n, grads, counts, types, outs, max_norm, eps, (const double*)workspace, partials, norm, s);
   });
 }
