@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "backend/pl_internal.h"
@@ -106,13 +107,24 @@ constexpr int H_BK = 64;   // panel depth of the 16-bit product
 // but for its ends); of 128 x 128 tiles, two per unit, 5 + 0.0136 K, or with one per unit 3.5 + 0.0069 K; a call 4.  Slices go
 // out in 32 bits and come back through a pass at about 4 TB/s, a launch of its own.
 struct HalfPlan { int tile, splits, kchunk; };   // tile 0: rows of fewer than 8 elements
+// Those: a thread per element of the product, so a long K is split until the threads fill the device; a slice of kc costs
+// its thread a wait per eight k, and the pass one per four slices, which are least together at kc near sqrt(2 K).
+inline HalfPlan plan_thin(long M, long N, long K) {
+  const long threads = 1L << 19, most = threads / (M * N > 0 ? M * N : 1);
+  long kc = (long)std::sqrt(2.0 * (double)K);
+  if (kc < 64) kc = 64;
+  if (most > 0 && kc < K / most) kc = K / most;
+  kc = whole(kc, 8);
+  const long s = (K + kc - 1) / kc;
+  return most < 2 || s < 2 ? HalfPlan{0, 1, 0} : HalfPlan{0, (int)s, (int)kc};
+}
 inline double half_rounds_us(int tile, long blocks, double k) {
   if (tile == 256) return (double)((blocks + 255) / 256) * (10.0 + 0.0222 * k);
   const long rem = blocks % 512;
   return (double)(blocks / 512) * (5.0 + 0.0136 * k) + (rem == 0 ? 0.0 : rem <= 256 ? 3.5 + 0.0069 * k : 5.0 + 0.0136 * k);
 }
 inline HalfPlan plan_half(bool at, bool bt, long M, long N, long K) {
-  if ((at ? K : M) < 8 || (bt ? N : K) < 8) return {0, 1, 0};
+  if ((at ? K : M) < 8 || (bt ? N : K) < 8) return plan_thin(M, N, K);
   HalfPlan best = {128, 1, 0};
   double best_us = 1e30;
   const unsigned k = (unsigned)K;

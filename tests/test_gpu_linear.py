@@ -373,6 +373,49 @@ def test_few_columns_of_unaligned_operands(pkg, L, kind, M, N, K):
     exact_product(pkg, L, kind, "T", "N", M, N, K, Layout(pad=1), kind_d="f32", seed=4)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("ta,tb,M,N,K", [("N", "T", 4096, 1, 16384), ("N", "T", 770, 7, 20001), ("T", "T", 300, 3, 17000), ("T", "T", 9, 1, 100003), ("N", "N", 5, 300, 16391),
+                                         ("N", "T", 3, 2, 65537), ("N", "N", 1, 64, 500), ("N", "T", 2, 5, 129), ("T", "N", 300, 200, 7), ("N", "N", 7, 70001, 65)])
+def test_products_of_rows_below_eight_elements(pkg, L, kind, ta, tb, M, N, K):
+    """The weight gradient of a head with one to seven outputs over many tokens, and its like: K in slices, exact on whole
+    numbers, close on normal ones, with nothing behind the workspace."""
+    for lay in (Layout(), Layout(pad=1), Layout(pad=3, offset=5)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay, kind_d="f32")
+    opA, opB, bias, Cm = rand(M, K, 5, kind, 2.0 * K ** -0.5), rand(K, N, 6, kind), rand(M, 1, 7, kind)[:, 0], rand(M, N, 8, "f32")
+    z, ez, y, ey = forward(opA, opB, bias, Cm, 1.25, -0.5, "silu", kind, "f32")
+    got, zs = product(pkg, L, kind, ta, tb, opA, opB, alpha=1.25, beta=-0.5, bias=bias, name="silu", keep=True, Cm=Cm, kind_d="f32")
+    check(zs, z, ez, "z")
+    check(got, y, ey, "y")
+    Z = rand(M, N, 33, kind, 2.0)
+    d, ed, db, edb = gradient(opA, opB, Z, None, 1.0, 0.0, "gelu", kind)
+    got, gdb = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="gelu", lay=Layout(pad=1))
+    check(got, d, ed, "D")
+    check(gdb, db, edb, "dbias")
+
+
+def test_the_gradient_of_one_output_costs_no_more_than_that_of_eight(pkg, L):
+    """4096 features, 16384 tokens, into fp32: rows of one element are no 16-byte vectors, and were summed by one thread per
+    element over all tokens (1346 us against 37)."""
+    M, K = 4096, 16384
+    x = torch.randn(K, M, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").bfloat16()
+    ep, best = pkg.epilogue(type_d=TYPES["f32"]), {}
+    for N in (1, 7, 8):
+        dy, g = torch.randn(K, N, device="cuda").bfloat16(), torch.zeros(N, M, device="cuda")
+        need = L.pl_gemm_epilogue_workspace_bytes(3, b"N", b"T", M, N, K, 0)
+        ws, times = workspace(need), []
+        for _ in range(8):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            pkg.check(L.pl_gemm_epilogue(3, b"N", b"T", M, N, K, 1.0, x.data_ptr(), M, dy.data_ptr(), N, C.byref(ep), 0.0, None, 0, g.data_ptr(), M, ws.data_ptr(), need,
+                                         stream()), "pl_gemm_epilogue")
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        best[N] = min(times[2:])
+    print(best, flush=True)
+    assert best[1] <= 3 * best[8] and best[7] <= 5 * best[8]
+
+
 @pytest.mark.parametrize("kind", ["f32", "f64"])
 @pytest.mark.parametrize("ta,tb", TRANS)
 @pytest.mark.parametrize("M,N,K", [(256, 256, 4096), (1700, 1500, 1600), (700, 300, 1001)])
