@@ -30,9 +30,9 @@ inline Workspace workspace_for(int type, const HalfPlan& p, const WidePlan& wp, 
     // the slices of a product alone on the device, or the product and behind it the slices of its tail; of the operands and
     // of their copies, whichever the call will be given
     const char ta = at ? 'T' : 'N', tb = bt ? 'T' : 'N';
-    long slices = product_alone_slices_bytes((int)wide, ta, tb, M, N, K);
+    long slices = product_alone_slices_bytes((int)wide, ta, tb, M, N, K, M, N);
     if (copies.bytes() > 0) {
-      const long padded = product_alone_slices_bytes((int)wide, ta, tb, M, N, whole(K, WIDE_K));
+      const long padded = product_alone_slices_bytes((int)wide, ta, tb, M, N, whole(K, WIDE_K), whole(M, WIDE_ROWS), whole(N, WIDE_ROWS));
       if (padded > slices) slices = padded;
     }
     w.product = round16(M * N * wide) + round16(slices);

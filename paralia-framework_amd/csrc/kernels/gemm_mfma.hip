@@ -1241,18 +1241,20 @@ int launch_gemm(char ta, char tb, long M, long N, long K, T alpha, const T* A, l
 #define PLK_ALONE_MAX_WS_BYTES (1L << 30)
 
 // What the linear layers' launcher asks and calls, under the built-in fit.
-// A product alone on the device, beta == 0: its predicted time with a workspace of ws_bytes, and the slices it needs.
+// A product alone on the device, beta == 0, whose operands may be read to m_read rows and n_read columns: its predicted time
+// with a workspace of ws_bytes, and the slices it needs.
 template <typename T>
-TileChoice fixed_choice(char ta, char tb, long M, long N, long K, long ws_bytes) {
+TileChoice fixed_choice(char ta, char tb, long M, long N, long K, long m_read, long n_read, long ws_bytes) {
   const bool an = ta == 'N' || ta == 'n', bnn = tb == 'N' || tb == 'n';
-  return choose_tile<T>(an, bnn, M, N, K, true, ws_bytes > 0, ws_bytes, true, 0, true, 0, 0, false, &fit_builtin());
+  return choose_tile<T>(an, bnn, M, N, K, true, ws_bytes > 0, ws_bytes, true, 0, true, m_read, n_read, false, &fit_builtin());
 }
-double product_alone_us(int elem_size, char ta, char tb, long M, long N, long K, long ws_bytes) {
-  return elem_size == 8 ? fixed_choice<double>(ta, tb, M, N, K, ws_bytes).us : fixed_choice<float>(ta, tb, M, N, K, ws_bytes).us;
+double product_alone_us(int elem_size, char ta, char tb, long M, long N, long K, long m_read, long n_read, long ws_bytes) {
+  return elem_size == 8 ? fixed_choice<double>(ta, tb, M, N, K, m_read, n_read, ws_bytes).us : fixed_choice<float>(ta, tb, M, N, K, m_read, n_read, ws_bytes).us;
 }
-long product_alone_slices_bytes(int elem_size, char ta, char tb, long M, long N, long K) {
+long product_alone_slices_bytes(int elem_size, char ta, char tb, long M, long N, long K, long m_read, long n_read) {
   if (K <= 0) return 0;
-  const TileChoice c = elem_size == 8 ? fixed_choice<double>(ta, tb, M, N, K, PLK_ALONE_MAX_WS_BYTES) : fixed_choice<float>(ta, tb, M, N, K, PLK_ALONE_MAX_WS_BYTES);
+  const TileChoice c = elem_size == 8 ? fixed_choice<double>(ta, tb, M, N, K, m_read, n_read, PLK_ALONE_MAX_WS_BYTES)
+                                      : fixed_choice<float>(ta, tb, M, N, K, m_read, n_read, PLK_ALONE_MAX_WS_BYTES);
   if (c.tail_splits > 1) return (long)c.tail_splits * M * (N - c.n_head) * elem_size;
   return c.splits > 1 ? (long)c.splits * M * N * elem_size : 0;
 }

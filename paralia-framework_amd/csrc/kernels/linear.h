@@ -62,9 +62,10 @@ inline bool same_or_apart(const Range& a, const Range& b) {
 }
 
 // gemm_mfma.hip: the fp32 / fp64 product alone on the device, all under the tile GEMM's built-in constants, so that neither a
-// database that is loaded later nor the environment changes a plan.  Its predicted time and the slices it needs,
-double product_alone_us(int elem_size, char ta, char tb, long M, long N, long K, long ws_bytes);
-long product_alone_slices_bytes(int elem_size, char ta, char tb, long M, long N, long K);
+// database that is loaded later nor the environment changes a plan.  Its predicted time and the slices it needs, its operands
+// readable to m_read rows and n_read columns,
+double product_alone_us(int elem_size, char ta, char tb, long M, long N, long K, long m_read, long n_read, long ws_bytes);
+long product_alone_slices_bytes(int elem_size, char ta, char tb, long M, long N, long K, long m_read, long n_read);
 // the product itself,
 int product_alone_f32(char ta, char tb, long M, long N, long K, float alpha, const void* A, long lda, const void* B, long ldb, float beta, void* C, long ldc, void* ws,
                       long ws_bytes, long m_read, long n_read, hipStream_t stream);
@@ -151,14 +152,48 @@ inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
   return p.splits > 1 || p.tile == 0 ? epilogue_pass_rows(type, M, N) : 2 * ((N + p.tile - 1) / p.tile);
 }
 
+// Space of the aligned copies of both operands, and their leading dimensions.
+struct Copies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
+
+// fp32 and fp64 operands that are unaligned or ragged are multiplied from copies, because their tile GEMM takes panels straight into LDS only from 16-byte aligned vectors and only in
+// whole tiles and panels: from aligned copies with k filled up by zeros to whole panels and rows to whole tiles of 256, an
+// unaligned product runs at nearly the full rate (3878 x 1869 x 4113 with odd strides, fp32 TN / NN / NT / TT: 970 / 900 /
+// 781 / 900 -> 537 / 506 / 507 / 506 us, fp64 1092 - 1190 -> 1010 - 1080), and of aligned operands with ragged edges loses
+// less (3880 x 1872 x 4112: fp32 551 - 598 -> 504, fp64 1076 - 1130 -> 1000 - 1010).  Products that fill less of the device
+// lose less; below the copies' own time there are none.  The space is set aside for whole extents too: their rows may be
+// those of a wider matrix.
+constexpr long WIDE_ROWS = 256, WIDE_K = 32;
+inline bool wide_aligned(int es, const void* A, long lda, const void* B, long ldb) {
+  return aligned_to(A, 16) && aligned_to(B, 16) && lda % (16 / es) == 0 && ldb % (16 / es) == 0;
+}
+inline double wide_copy_us(int es, long kw, long mw, long nw) { return 10.0 + (double)es * (double)kw * (double)(2 * mw + 2 * nw) / 3e6; }
+inline Copies wide_copies(int es, bool aligned, bool at, bool bt, long M, long N, long K) {
+  Copies c = {0, 0, 0, 0};
+  if (K <= 0 || M > (1L << 28) || N > (1L << 28) || K > (1L << 28)) return c;
+  const bool ragged = M % 128 != 0 || N % 128 != 0 || K % WIDE_K != 0;
+  const double product_us = 2.0 * (double)M * (double)N * (double)K / (es == 4 ? 138e6 : 72e6);
+  const double gain = !aligned ? (es == 4 ? 0.6 : 0.25) : ragged ? (es == 4 ? 0.15 : 0.1) : 0.0;
+  const long kw = whole(K, WIDE_K), mw = whole(M, WIDE_ROWS), nw = whole(N, WIDE_ROWS);
+  if (gain * product_us < wide_copy_us(es, kw, mw, nw)) return c;
+  c.ld_a = at ? kw : mw;
+  c.ld_b = bt ? nw : kw;
+  c.bytes_a = (at ? mw : kw) * c.ld_a * es;
+  c.bytes_b = (bt ? kw : nw) * c.ld_b * es;
+  return c;
+}
+
 // How an fp32 or fp64 product is launched: in the tile GEMM's tiles with the epilogue as a pass (splits 0), or in 64 x 64 tiles
 // with the epilogue inside, K split `splits` ways where it is long.  A function of the shape and the type alone.  Times in
 // microseconds, fitted to 216 products of 64 x 64 x 64 to 8192 x 2048 x 2048: a 64 x 64 tile alone on its unit takes 0.053
 // (fp32 0.032) per k, several on one 0.039 (0.0245) each, and 1 (0.5) for its epilogue; a pass over slices 3, and for each
 // slice 0.8 and its bytes at 5.7 TB/s (the memory-side cache holds them).  The rule's choices are 1 % from the best of all
-// measured ones, the tile GEMM's 24 %.
+// measured ones, the tile GEMM's 24 %.  The tile GEMM is priced as the call would run it: from copies, where it makes them
+// (priced by its rate on unaligned operands, large fp32 products of odd extents went to 64 x 64 tiles, up to 1.5 x behind;
+// over 187 odd and ragged shapes both ways the choices are now 0.7 % from the better one, at worst 1.16 x).
 // Both sides, fp64 / fp32, tile GEMM -> 64 x 64: 605 x 195 x 174 38 / 30 -> 16 / 11, 9472 x 192 x 3 21 / 17 -> 11 / 8,
 // 10474 x 17 x 2943 170 / 105 -> 99 / 66; 2048 x 2048 x 512 79 / 44 -> 87 / 54, 2048^3 256 / 133 -> 318 / 192.
+// Odd extents, copies / 64 x 64, fp32: 3878 x 1869 x 4113 506 - 552 / 699 - 776, 829 x 10936 x 2184 NT 378 / 502,
+// 2253 x 1029 x 2616 132 / 180; 1501 x 1301 x 2003 103 / 99, 320 x 2293 x 1536 46 / 41.
 struct WidePlan { int splits, kchunk; };
 inline WidePlan plan_wide(int es, bool at, bool bt, long M, long N, long K) {
   if (M > (1L << 27) || N > (1L << 27) || K > (1L << 30)) return {0, 0};
@@ -180,9 +215,14 @@ inline WidePlan plan_wide(int es, bool at, bool bt, long M, long N, long K) {
     if (us < best_us) best_us = us, best = {s, s > 1 ? kc : 0};
   }
   if (best_us < 10.0 || K == 0) return best;   // (less than the tile GEMM's two launches ever take)
+  // the tile GEMM as the call would run it: from copies, which are readable to the tiles' edges, where it makes them
+  const char ta = at ? 'T' : 'N', tb = bt ? 'T' : 'N';
   const long per = 16 / es;
   const bool unaligned = (at ? K : M) % per != 0 || (bt ? N : K) % per != 0, ragged = M % 128 != 0 || N % 128 != 0 || K % 32 != 0;
-  const double gemm = product_alone_us(es, at ? 'T' : 'N', bt ? 'T' : 'N', M, N, K, 1L << 28) * (unaligned ? (es == 4 ? 1.6 : 1.25) : ragged ? 1.1 : 1.0);
+  const long kw = whole(K, WIDE_K), mw = whole(M, WIDE_ROWS), nw = whole(N, WIDE_ROWS);
+  const double gemm = wide_copies(es, !unaligned, at, bt, M, N, K).bytes() > 0
+                          ? product_alone_us(es, ta, tb, M, N, kw, mw, nw, 1L << 28) + wide_copy_us(es, kw, mw, nw)
+                          : product_alone_us(es, ta, tb, M, N, K, M, N, 1L << 28) * (unaligned ? (es == 4 ? 1.6 : 1.25) : ragged ? 1.1 : 1.0);
   return best_us < 0.95 * (2.0 + gemm + 2.0 * cells_us) ? best : WidePlan{0, 0};
 }
 int wide_product_f32(const Call& c, const WidePlan& plan, bool at, bool bt, const Epilogue& ep, void* slices);
@@ -200,7 +240,6 @@ inline bool can_request(const void* A, long lda, const void* B, long ldb) {
 // panels are loaded by every tile in its row or column, and the copies cost one launch and one pass over the operands
 // (4100 x 1023 x 2052, rows of an odd number of elements: 70 -> 47 us).  The space is set aside by the shape alone: where a
 // contiguous extent is no multiple of 8, so that dense operands could not be aligned.
-struct Copies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
 inline Copies half_copies(bool at, bool bt, long M, long N, long K) {
   const long ext_a = at ? K : M, rows_a = at ? M : K, ext_b = bt ? N : K, rows_b = bt ? K : N;
   Copies c = {0, 0, 0, 0};
@@ -216,31 +255,6 @@ inline Copies half_copies(bool at, bool bt, long M, long N, long K) {
   return c;
 }
 
-// The same for fp32 and fp64, whose tile GEMM takes panels straight into LDS only from 16-byte aligned vectors and only in
-// whole tiles and panels: from aligned copies with k filled up by zeros to whole panels and rows to whole tiles of 256, an
-// unaligned product runs at nearly the full rate (3878 x 1869 x 4113 with odd strides, fp32 TN / NN / NT / TT: 970 / 900 /
-// 781 / 900 -> 537 / 506 / 507 / 506 us, fp64 1092 - 1190 -> 1010 - 1080), and of aligned operands with ragged edges loses
-// less (3880 x 1872 x 4112: fp32 551 - 598 -> 504, fp64 1076 - 1130 -> 1000 - 1010).  Products that fill less of the device
-// lose less; below the copies' own time there are none.  The space is set aside for whole extents too: their rows may be
-// those of a wider matrix.
-constexpr long WIDE_ROWS = 256, WIDE_K = 32;
-inline bool wide_aligned(int es, const void* A, long lda, const void* B, long ldb) {
-  return aligned_to(A, 16) && aligned_to(B, 16) && lda % (16 / es) == 0 && ldb % (16 / es) == 0;
-}
-inline Copies wide_copies(int es, bool aligned, bool at, bool bt, long M, long N, long K) {
-  Copies c = {0, 0, 0, 0};
-  if (K <= 0 || M > (1L << 28) || N > (1L << 28) || K > (1L << 28)) return c;
-  const bool ragged = M % 128 != 0 || N % 128 != 0 || K % WIDE_K != 0;
-  const double product_us = 2.0 * (double)M * (double)N * (double)K / (es == 4 ? 138e6 : 72e6);
-  const double gain = !aligned ? (es == 4 ? 0.6 : 0.25) : ragged ? (es == 4 ? 0.15 : 0.1) : 0.0;
-  const long kw = whole(K, WIDE_K), mw = whole(M, WIDE_ROWS), nw = whole(N, WIDE_ROWS);
-  if (gain * product_us < 10.0 + (double)es * (double)kw * (double)(2 * mw + 2 * nw) / 3e6) return c;
-  c.ld_a = at ? kw : mw;
-  c.ld_b = bt ? nw : kw;
-  c.bytes_a = (at ? mw : kw) * c.ld_a * es;
-  c.bytes_b = (bt ? kw : nw) * c.ld_b * es;
-  return c;
-}
 int copy_operands(int es, const void* A, long lda, void* copy_a, const void* B, long ldb, void* copy_b, const Call& c, bool at, bool bt, const Copies& to);
 
 // few columns of two K-major operands that can be requested, in whole panels of k: a kernel of their own

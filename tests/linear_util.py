@@ -160,3 +160,12 @@ def shipped_fit(pkg, L):
         elif name in fields:
             setattr(f, name, float(value))
     return f
+
+
+def takes_copies(L, kind, ta, tb, M, N, K):
+    """Whether an fp32 or fp64 product sets space aside for aligned copies of its operands: behind the product, rows in whole
+    tiles of 256 and k in whole panels of 32."""
+    up = lambda n, unit: -(-n // unit) * unit  # noqa: E731
+    es = 8 if kind == "f64" else 4
+    need = L.pl_gemm_epilogue_workspace_bytes(TYPES[kind], ta.encode(), tb.encode(), M, N, K, 0)
+    return need >= M * N * es + (up(M, 256) + up(N, 256)) * up(K, 32) * es

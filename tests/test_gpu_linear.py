@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from linear_util import ACTS, TORCH, TYPES, Mat, check, forward, gradient, half_step, shipped_fit, slope_product
+from linear_util import ACTS, TORCH, TYPES, Mat, check, forward, gradient, half_step, shipped_fit, slope_product, takes_copies
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -441,6 +441,25 @@ def test_wide_products_of_unaligned_operands(pkg, L, kind, ta, tb, M, N, K):
     opA, opB, Cm = rand_ints(M, K, 7), rand_ints(K, N, 8), rand_ints(M, N, 9, -9, 9)
     got, _ = product(pkg, L, kind, ta, tb, opA, opB, alpha=2.0, beta=-1.0, Cm=Cm, in_place=True, lay=Layout(pad=1))
     assert torch.equal(got, 2.0 * (opA @ opB) - Cm)
+    opA, opB, Z = rand(M, K, 31, kind, K ** -0.5), rand(K, N, 32, kind), rand(M, N, 33, kind, 2.0)
+    d, ed, db, edb = gradient(opA, opB, Z, None, 1.0, 0.0, "gelu_tanh", kind)
+    got, gdb = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="gelu_tanh", lay=Layout(pad=1))
+    check(got, d, ed, "D")
+    check(gdb, db, edb, "dbias")
+
+
+@pytest.mark.parametrize("kind,M,N,K", [("f32", 2061, 1803, 1003), ("f32", 3400, 1809, 424), ("f32", 2100, 2052, 1500), ("f64", 2305, 2305, 1301)])
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_wide_products_from_copies(pkg, L, kind, ta, tb, M, N, K):
+    """Products that do set space aside for copies, none with a K of whole panels: what fills it up has to count as zero,
+    whatever lies behind the operands' rows and in the workspace (NaN, both)."""
+    assert takes_copies(L, kind, ta, tb, M, N, K) and K % 32 != 0
+    for lay in (Layout(), Layout(pad=1), Layout(pad=3, offset=1), Layout(pad=4)):
+        exact_product(pkg, L, kind, ta, tb, M, N, K, lay)
+    opA, opB, Cm = rand_ints(M, K, 7), rand_ints(K, N, 8), rand_ints(M, N, 9, -9, 9)
+    for lay in (Layout(), Layout(pad=1)):
+        got, _ = product(pkg, L, kind, ta, tb, opA, opB, alpha=2.0, beta=-1.0, Cm=Cm, in_place=True, lay=lay)   # (nothing but the product)
+        assert torch.equal(got, 2.0 * (opA @ opB) - Cm)
     opA, opB, Z = rand(M, K, 31, kind, K ** -0.5), rand(K, N, 32, kind), rand(M, N, 33, kind, 2.0)
     d, ed, db, edb = gradient(opA, opB, Z, None, 1.0, 0.0, "gelu_tanh", kind)
     got, gdb = product_grad(pkg, L, kind, ta, tb, opA, opB, Z, name="gelu_tanh", lay=Layout(pad=1))

@@ -5,7 +5,7 @@ import random
 
 import pytest
 
-from linear_util import shipped_fit
+from linear_util import shipped_fit, takes_copies
 
 A, B, CM, D, Z, DB, WS = (0x10000000 * i for i in range(1, 8))   # addresses nobody dereferences
 
@@ -185,3 +185,15 @@ def test_the_workspace_is_a_function_of_the_shape_alone(pkg, L, monkeypatch):
         with monkeypatch.context() as m:
             m.setenv(name, value)
             assert ask() == before, (name, value)
+
+
+@pytest.mark.parametrize("ta", ["N", "T"])
+@pytest.mark.parametrize("tb", ["N", "T"])
+def test_which_products_are_multiplied_from_copies(L, ta, tb):
+    """Measured on 68 shapes both ways: large products of odd extents are faster from copies in the tile GEMM's tiles, small and
+    narrow ones in 64 x 64 tiles."""
+    for kind, M, N, K in (("f32", 3878, 1869, 4113), ("f32", 829, 10936, 2184), ("f32", 10936, 829, 2184), ("f32", 2253, 1029, 2616), ("f32", 3400, 1809, 424),
+                          ("f32", 5991, 921, 5269), ("f32", 2061, 6226, 1334), ("f64", 3878, 1869, 4113), ("f64", 5510, 4977, 663)):
+        assert takes_copies(L, kind, ta, tb, M, N, K), (kind, M, N, K)
+    for kind, M, N, K in (("f32", 605, 195, 174), ("f64", 605, 195, 174), ("f32", 10474, 17, 2943), ("f64", 2304, 300, 1024), ("f32", 4893, 190, 1539)):
+        assert not takes_copies(L, kind, ta, tb, M, N, K), (kind, M, N, K)
