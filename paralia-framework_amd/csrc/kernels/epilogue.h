@@ -75,8 +75,8 @@ __device__ __forceinline__ void store_row(T* p, const W (&v)[N], int valid) {
 }
 
 // ---- activations ----
-// Accuracy classes: F16 (results rounded to 16 bits: relative error below 1e-5, which a rounding to 2^-11 or 2^-8 hides),
-// and the full precision of W for 32 and 64 bits.
+// Accuracy classes: FAST for results rounded to 16 bits (relative error below 1e-5, which a rounding to 2^-11 or 2^-8 hides),
+// and the full precision of W for results in 32 and 64 bits, those of 16-bit operands among them.
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
@@ -227,7 +227,7 @@ template <typename T, typename TD, bool GRAD, int VEC>
 __device__ __forceinline__ void apply_epilogue(const Epilogue& ep, const EpilogueInputs<T, TD, GRAD, VEC>& in, wide_t<T> (&v)[VEC], const wide_t<T> (&bias)[VEC], TD* pd,
                                                T* pp, int valid, wide_t<T> (&sums)[VEC]) {
   using W = wide_t<T>;
-  constexpr bool FAST = sizeof(T) == 2;
+  constexpr bool FAST = sizeof(T) == 2 && sizeof(TD) == 2;   // (an fp32 D shows the short forms: gelu near 0 24 against 3 units of 2^-24)
   const W alpha = (W)ep.alpha, beta = (W)ep.beta;
   int act = ep.act;
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from linear_util import ACTS, TORCH, TYPES, Mat, check, forward, gradient, half_step, shipped_fit, slope_product, takes_copies
+from linear_util import ACTS, TORCH, TYPES, Mat, act, act_error, check, forward, gradient, half_step, shipped_fit, slope_product, takes_copies
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -149,6 +149,25 @@ def test_activations(pkg, L, kind, name, M, N, K):
         got, _ = product(pkg, L, kind, "T", "N", opA, opB, bias=bias, name=name, kind_d="f32")
         z, ez, y, ey = forward(opA, opB, bias, None, 1.0, 0.0, name, kind, "f32")
         check(got, y, ey, "y in 32 bits")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("ta,tb,M,N,K", [("T", "N", 300, 2, 64), ("N", "N", 300, 80, 64), ("T", "T", 2048, 2048, 72), ("N", "N", 256, 256, 4096), ("N", "N", 300, 9, 3)])
+def test_activations_into_32_bits(pkg, L, kind, name, ta, tb, M, N, K):
+    """An fp32 D of 16-bit operands shows what 16 bits would hide: the activation of an exact z to the accuracy of fp32 (few
+    columns, tiles, large tiles, slices, thin rows)."""
+    z = torch.linspace(-9.0, 9.0, M, dtype=torch.float64, device="cuda").to(TORCH[kind]).double()
+    opA, opB = torch.zeros(M, K, dtype=torch.float64, device="cuda"), torch.zeros(K, N, dtype=torch.float64, device="cuda")
+    opA[:, 1], opB[1] = z, 1.0
+    got, _ = product(pkg, L, kind, ta, tb, opA, opB, name=name, kind_d="f32")
+    y, bound = act(z, name), act_error(z, name, "f32")
+    if name == "gelu":
+        # (torch's ndtr loses the lower tail, -9 Phi(-9) = -1.0157e-18; erfc keeps it.)  u = 2^-24: 4 for an erfc of 2 ulp, 2 (1 + z^2) for the
+        # two roundings of its argument, 1 for the product
+        y, bound = z * 0.5 * torch.erfc(z * -0.5 ** 0.5), (8 + 2 * z * z) * 2.0 ** -24
+    y, bound = y[:, None].expand(M, N), bound[:, None]
+    check(got, y, bound * y.abs() + half_step(y, "f32"), "y")
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16", "f32", "f64"])
