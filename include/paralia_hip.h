@@ -259,7 +259,8 @@ int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K,
 
 /* D <- (alpha*op(A)*op(B) + beta*C) .* act'(Z), the gradient that a following layer's product sends back through this
  * layer's activation, Z being what pl_gemm_epilogue left in preact; dbias(m) <- sum over n of D(m, n) before its
- * rounding (null: not wanted; M elements).  relu'(0) is 0.  PL_ACT_NONE does not read Z.  D may be C or Z itself.
+ * rounding (null: not wanted; M elements).  relu'(0) is 0, and what arrives where relu' is 0, infinities and NaN too,
+ * leaves a 0.  PL_ACT_NONE does not read Z.  D may be C or Z itself.
  * workspace: as above, with_dbias = 1 where dbias is given. */
 int pl_gemm_epilogue_grad(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda,
                           const void* B, long ldb, int activation, const void* Z, long ldz, double beta, const void* C, long ldc,

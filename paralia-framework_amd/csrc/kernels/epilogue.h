@@ -160,7 +160,7 @@ template <typename W, bool FAST, int VEC> __device__ __forceinline__ void activa
 template <typename W, bool FAST, int VEC> __device__ __forceinline__ void times_slope(W (&v)[VEC], const W (&zs)[VEC], int act) {
   if (act == PL_ACT_RELU) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = zs[e] > W(0) ? v[e] : v[e] * W(0);
+    for (int e = 0; e < VEC; ++e) v[e] = zs[e] > W(0) ? v[e] : W(0);   // (not times 0: infinities and NaN stay out too)
   } else if (act == PL_ACT_GELU) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {

@@ -267,6 +267,31 @@ def test_infinities_and_nan_go_where_the_formula_sends_them(pkg, L, kind):
     assert torch.equal(got[keep], clean[keep])
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32", "f64"])
+def test_a_closed_relu_lets_nothing_through(pkg, L, kind):
+    """Infinite and NaN gradients where z <= 0 are zeros of D and add nothing to dbias; where z > 0 they arrive."""
+    M, N, K = 150, 70, 40
+    g, Z = rand_ints(M, N, 1, 1, 9), rand_ints(M, N, 2, -3, 3)
+    closed = Z <= 0
+    bad = g.clone()
+    bad[closed & (rand_ints(M, N, 3) > 0)] = float("inf")
+    bad[closed & (rand_ints(M, N, 3) < 0)] = NAN
+    want = torch.where(closed, torch.zeros_like(g), g)
+    for lay, in_place in ((Layout(), None), (Layout(pad=3, offset=1), None), (Layout(), "dY"), (Layout(), "Z")):
+        got, db = act_grad(pkg, L, kind, "relu", bad, Z, lay=lay, in_place=in_place)
+        assert torch.equal(got, want) and torch.equal(db, want.sum(1).to(TORCH[kind]).double())
+    # the same arriving in C, in front of a product
+    opA, opB = rand_ints(M, K, 4), rand_ints(K, N, 5)
+    want = torch.where(closed, torch.zeros_like(g), g + opA @ opB)
+    got, db = product_grad(pkg, L, kind, "T", "N", opA, opB, Z, beta=1.0, Cm=bad, name="relu")
+    assert torch.equal(got, want.to(TORCH[kind]).double()) and torch.equal(db, want.sum(1).to(TORCH[kind]).double())
+    open_ = g.clone()
+    m, n = (Z > 0).nonzero()[0].tolist()
+    open_[m, n] = float("inf")
+    got, db = act_grad(pkg, L, kind, "relu", open_, Z)
+    assert torch.isinf(got[m, n]) and torch.isinf(db[m]) and int(torch.isinf(got).sum()) == 1
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_alpha_zero_and_k_zero_do_not_read_the_operands(pkg, L, kind):
     M, N = 70, 50
