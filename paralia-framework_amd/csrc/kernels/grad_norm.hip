@@ -121,8 +121,11 @@ __global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(const double* _
   if (threadIdx.x == 0) *norm = r;
 }
 
+// The factor is rounded to 32 bits for elements of 32 and 16 (half a unit of 2^-24 that the element's own rounding joins),
+// but where it is below their normal numbers, and would lose bits or vanish, the product is formed in 64.
 template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T* q, int count, double scale) {
   const wide_t<T> f = (wide_t<T>)scale;
+  const bool tiny = sizeof(wide_t<T>) == 4 && scale < 0x1p-126;
 #pragma unroll
   for (int i = 0; i < CHUNK / (8 * NORM_THREADS); ++i) {
     const int at = (i * NORM_THREADS + (int)threadIdx.x) * 8;
@@ -130,8 +133,13 @@ template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T*
     if (valid > 0) {
       wide_t<T> v[8];
       load_row<T, 8, wide_t<T>, true>(p + at, v, valid);
+      if (tiny) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= f;
+        for (int e = 0; e < 8; ++e) v[e] = (wide_t<T>)((double)v[e] * scale);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f;
+      }
       store_row<T, 8, wide_t<T>>(q + at, v, valid);
     }
   }

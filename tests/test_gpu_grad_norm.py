@@ -223,3 +223,21 @@ def test_a_long_list_costs_what_its_parts_cost(pkg, L):
     want = math.sqrt(float((flat.double() ** 2).sum()))
     assert abs(float(norm) - want) <= want * n * count * 2.0 ** -53
     assert together <= 1.5 * apart
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("limit", [1.0, 1e-3, 1e-6, 1e-30])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_factors_below_the_normal_numbers_of_32_bits(pkg, L, kind, limit, in_place):
+    """Gradients of 5e37 against a small limit: a factor that 32 bits hold in a few bits or not at all (1e-40 .. 1e-70) scales
+    like any other.  Bounds as above: factor and product in the wide type, then one rounding to the tensor's."""
+    t = Tensors([(1000, kind, 3), (20, "f64", 0)], 5, 5e37)
+    before = [v.double().clone() for v in t.views]
+    norm = t.norm()
+    assert abs(clip(pkg, L, t, limit, in_place) - norm) <= norm * 1024 * 2.0 ** -53
+    scale = limit / (norm + EPS)
+    assert scale < 2.0 ** -126
+    for v, o, b, k in zip(t.views, t.out_views, before, t.kinds):
+        want = b * scale
+        err = want.abs() * (2.0 ** -51 if k == "f64" else 2.0 ** -22) + want.abs() * 1024 * 2.0 ** -52
+        assert bool((((v if in_place else o).double() - want).abs() <= err + half_step(want.abs() + err, k)).all())
