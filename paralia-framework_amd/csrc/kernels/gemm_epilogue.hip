@@ -167,11 +167,13 @@ int run_product(Call& c) {
     const bool f64 = c.type == PL_TYPE_F64;
     if (plain_product(c)) {
       // nothing but the product (and C where D is): the tile GEMM's own epilogue
-      return f64 ? product_alone_f64(c.ta, c.tb, M, N, c.K, ep.alpha, c.A, c.lda, c.B, c.ldb, ep.beta, ep.D, ep.ldd, ws, w.product, m_read, n_read, c.stream)
-                 : product_alone_f32(c.ta, c.tb, M, N, c.K, (float)ep.alpha, c.A, c.lda, c.B, c.ldb, (float)ep.beta, ep.D, ep.ldd, ws, w.product, m_read, n_read, c.stream);
+      rc_ = f64 ? product_alone_f64(c.ta, c.tb, M, N, c.K, ep.alpha, c.A, c.lda, c.B, c.ldb, ep.beta, ep.D, ep.ldd, ws, w.product, m_read, n_read, c.stream)
+                : product_alone_f32(c.ta, c.tb, M, N, c.K, (float)ep.alpha, c.A, c.lda, c.B, c.ldb, (float)ep.beta, ep.D, ep.ldd, ws, w.product, m_read, n_read, c.stream);
+      return rc_ == PL_ERR_LAUNCH ? refuse(rc_, who, "kernel launch failed") : rc_;
     }
     int slices = 1;
     rc_ = (f64 ? product_slices_f64 : product_slices_f32)(c.ta, c.tb, M, N, c.K, c.A, c.lda, c.B, c.ldb, ws, w.product, m_read, n_read, f64 && c.grad, &slices, c.stream);
+    if (rc_ == PL_ERR_LAUNCH) return refuse(rc_, who, "kernel launch failed");
     if (rc_ == PL_OK) rc_ = epilogue_pass(c.type, c.type_d, c.grad, M, N, ws, M, M * N, slices, ep, c.stream);
   }
   if (rc_ != PL_OK || !c.dbias) return rc_;

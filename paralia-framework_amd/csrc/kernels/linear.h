@@ -14,15 +14,6 @@
 
 namespace plk {
 
-// A launch without the triple-chevron's detour, arguments by reference: 128 tensors are 3.6 KB of them.
-template <typename... P>
-int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, const std::type_identity_t<P>&... args) {
-  void* list[] = {const_cast<void*>(static_cast<const void*>(&args))...};
-  if (hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, 0, stream) == hipSuccess) return PL_OK;
-  (void)hipGetLastError();   // (reported here, not by the caller's next call)
-  return PL_ERR_LAUNCH;
-}
-
 inline bool valid_type(int t) { return t >= PL_TYPE_F64 && t <= PL_TYPE_BF16; }
 inline bool valid_act(int a) { return a >= PL_ACT_NONE && a <= PL_ACT_SILU; }
 inline int type_size(int t) { return t == PL_TYPE_F64 ? 8 : t == PL_TYPE_F32 ? 4 : 2; }
@@ -32,6 +23,16 @@ inline int refuse(int code, const char* who, const char* why) {
   char text[200];
   snprintf(text, sizeof(text), "%s: %s", who, why);
   return pl_fail_msg(code, text);
+}
+
+// A launch without the triple-chevron's detour, arguments by reference: 128 tensors are 3.6 KB of them.
+template <typename... P>
+int launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, const std::type_identity_t<P>&... args) {
+  void* list[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, 0, stream);
+  if (e == hipSuccess) return PL_OK;
+  (void)hipGetLastError();   // (reported here, not by the caller's next call)
+  return refuse(PL_ERR_LAUNCH, "kernel launch", hipGetErrorString(e));
 }
 
 // A column-major operand's memory.

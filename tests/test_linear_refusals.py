@@ -197,3 +197,20 @@ def test_which_products_are_multiplied_from_copies(L, ta, tb):
         assert takes_copies(L, kind, ta, tb, M, N, K), (kind, M, N, K)
     for kind, M, N, K in (("f32", 605, 195, 174), ("f64", 605, 195, 174), ("f32", 10474, 17, 2943), ("f64", 2304, 300, 1024), ("f32", 4893, 190, 1539)):
         assert not takes_copies(L, kind, ta, tb, M, N, K), (kind, M, N, K)
+
+
+def test_a_failed_launch_says_so(pkg, L):
+    """Without a device every launch fails: the status says so and pl_last_error() is this call's, not an older one's."""
+    count = C.c_int(0)
+    if L.pl_device_count(C.byref(count)) == 0 and count.value > 0:
+        pytest.skip("a device would run kernels on these addresses")
+    big = 1 << 30
+    calls = {"few columns": lambda: call(L, pkg, K=64, lda=64, ldb=64), "tiles": lambda: call(L, pkg, ta=b"N", lda=64), "64 x 64": lambda: call(L, pkg, type=1),
+             "tile GEMM": lambda: call(L, pkg, type=0, M=2048, N=2048, K=2048, lda=2048, ldb=2048, ldd=2048, B=16 * B, D=32 * D, ws=64 * WS, wsb=big),
+             "its epilogue": lambda: call(L, pkg, type=0, act=1, M=2048, N=2048, K=2048, lda=2048, ldb=2048, ldd=2048, B=16 * B, D=32 * D, ws=64 * WS, wsb=big),
+             "gradient": lambda: grad(L), "activation": lambda: act_grad(L), "clipping": lambda: clip(L, [A, B], [100, 200], [1, 3], [A, B]),
+             "no columns": lambda: act_grad(L, N=0)}
+    for name, f in calls.items():
+        assert act_grad(L, type=-1) == 7 and b"unknown element type" in L.pl_last_error()
+        assert f() == 4, name
+        assert b"launch" in L.pl_last_error(), name
