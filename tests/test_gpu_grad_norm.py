@@ -241,3 +241,36 @@ def test_factors_below_the_normal_numbers_of_32_bits(pkg, L, kind, limit, in_pla
         want = b * scale
         err = want.abs() * (2.0 ** -51 if k == "f64" else 2.0 ** -22) + want.abs() * 1024 * 2.0 ** -52
         assert bool((((v if in_place else o).double() - want).abs() <= err + half_step(want.abs() + err, k)).all())
+
+
+def test_a_captured_long_list_replays(pkg, L):
+    """300 tensors whose norm is folded by a launch of its own: recorded, replayed on new gradients, norms and outputs bit for
+    bit those of the eager call, with nothing behind the workspace."""
+    n, count = 300, 70001
+    flat = torch.empty(n * count, device="cuda")
+    outs, norms = [torch.zeros_like(flat) for _ in range(2)], [torch.zeros(1, dtype=torch.float64, device="cuda") for _ in range(2)]
+    lists = [(C.c_void_p * n)(*[b.data_ptr() + 4 * count * i for i in range(n)]) for b in (flat, *outs)]
+    counts, types = (C.c_longlong * n)(*[count] * n), (C.c_int * n)(*[TYPES["f32"]] * n)
+    need = L.pl_grad_norm_workspace_bytes(n)
+    ws = [torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device="cuda") for _ in range(2)]
+
+    def call(i, s):
+        pkg.check(L.pl_grad_norm_clip(n, lists[0], counts, types, lists[1 + i], 1.0, EPS, norms[i].data_ptr(), ws[i].data_ptr(), need, s), "pl_grad_norm_clip")
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    flat.normal_(generator=g)
+    call(1, stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        call(1, torch.cuda.current_stream().cuda_stream)
+    for replay in range(4):
+        flat.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        call(0, stream())
+        torch.cuda.synchronize()
+        want = math.sqrt(float((flat.double() ** 2).sum()))
+        assert abs(float(norms[0]) - want) <= want * n * count * 2.0 ** -53
+        assert torch.equal(norms[0], norms[1]) and torch.equal(outs[0], outs[1]), replay
+        assert all(bool((w[need:] == 0xA5).all()) for w in ws)

@@ -755,3 +755,35 @@ def test_two_streams_and_two_threads_at_once(pkg, L):
         for a, b in zip(want, m.outputs()):
             assert torch.equal(a, b)
 
+
+
+@pytest.mark.parametrize("kind,ta,tb,M,N,K", [("bf16", "N", "T", 1030, 3, 9000), ("f16", "N", "N", 5, 300, 4100), ("f32", "T", "N", 2061, 1803, 1003), ("f64", "N", "T", 700, 300, 1001)])
+def test_captured_products_replay(pkg, L, kind, ta, tb, M, N, K):
+    """Slices of thin products, copies, 64 x 64 slices: recorded, replayed on new operands with eager calls and synchronisations
+    in between, bit for bit what the eager call leaves; nothing behind the workspace."""
+    need = L.pl_gemm_epilogue_workspace_bytes(TYPES[kind], ta.encode(), tb.encode(), M, N, K, 1)
+    A, B, Z = Mat(*((M, K) if ta == "N" else (K, M)), (M if ta == "N" else K) + 1, kind), Mat(*((K, N) if tb == "N" else (N, K)), (K if tb == "N" else N) + 1, kind), Mat(M, N, M, kind)
+    outs = [(Mat(M, N, M, kind, gap=7.0), Mat(M, 1, M, kind, gap=5.0), torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device="cuda")) for _ in range(2)]
+
+    def step(D, db, ws, s):
+        pkg.check(L.pl_gemm_epilogue_grad(TYPES[kind], ta.encode(), tb.encode(), M, N, K, 0.5, A.ptr, A.ld, B.ptr, B.ld, ACTS["silu"], Z.ptr, Z.ld, 0.0, None, 0, D.ptr, D.ld,
+                                          db.ptr, ws.data_ptr(), need, s), "pl_gemm_epilogue_grad")
+
+    def fill(seed):
+        A.set(rand(A.rows, A.cols, seed, kind)), B.set(rand(B.rows, B.cols, seed + 1, kind, K ** -0.5)), Z.set(rand(M, N, seed + 2, kind))
+
+    fill(1)
+    step(*outs[0], stream())
+    step(*outs[1], stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        step(*outs[1], torch.cuda.current_stream().cuda_stream)
+    for replay in range(4):
+        fill(10 * replay + 20)
+        graph.replay()
+        torch.cuda.synchronize()
+        step(*outs[0], stream())
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0][0].get(), outs[1][0].get()) and torch.equal(outs[0][1].get(), outs[1][1].get()), replay
+        assert all(bool((ws[need:] == 0xA5).all()) for _, _, ws in outs)
