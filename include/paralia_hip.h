@@ -251,7 +251,8 @@ typedef struct pl_epilogue {
  * take about twice as long, or are copied into the workspace first where a contiguous extent is no multiple of 8 elements
  * (the only case whose space is set aside) and the product is long enough.  fp32 and fp64 products that are large enough
  * for it are multiplied from copies laid out in whole tiles where an operand is not 16-byte aligned or an extent is ragged;
- * their space is always set aside. */
+ * their space is always set aside.  The size is a function of the arguments alone: neither pl_gemm_set_fit nor a routine
+ * that loads its database changes it. */
 long pl_gemm_epilogue_workspace_bytes(int type, char transA, char transB, long M, long N, long K, int with_dbias);
 int pl_gemm_epilogue(int type, char transA, char transB, long M, long N, long K, double alpha, const void* A, long lda, const void* B,
                      long ldb, const pl_epilogue* epilogue, double beta, const void* C, long ldc, void* D, long ldd, void* workspace,

@@ -159,7 +159,7 @@ struct Copies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return b
 // fp32 and fp64 operands that are unaligned or ragged are multiplied from copies, because their tile GEMM takes panels straight into LDS only from 16-byte aligned vectors and only in
 // whole tiles and panels: from aligned copies with k filled up by zeros to whole panels and rows to whole tiles of 256, an
 // unaligned product runs at nearly the full rate (3878 x 1869 x 4113 with odd strides, fp32 TN / NN / NT / TT: 970 / 900 /
-// 781 / 900 -> 537 / 506 / 507 / 506 us, fp64 1092 - 1190 -> 1010 - 1080), and of aligned operands with ragged edges loses
+// 781 / 900 -> 512 - 552 / 510 / 509 / 508 us, fp64 1092 - 1190 -> 1030), and of aligned operands with ragged edges loses
 // less (3880 x 1872 x 4112: fp32 551 - 598 -> 504, fp64 1076 - 1130 -> 1000 - 1010).  Products that fill less of the device
 // lose less; below the copies' own time there are none.  The space is set aside for whole extents too: their rows may be
 // those of a wider matrix.
