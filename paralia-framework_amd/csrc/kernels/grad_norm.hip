@@ -148,8 +148,8 @@ template <typename T> __device__ __forceinline__ void chunk_scale(const T* p, T*
 // partials > 0: every workgroup folds the partial sums of the norm's launches itself, in the same order (at most 16 KiB out
 // of the L2, against a launch of its own), and workgroup 0 of the first launch stores the norm.  partials == 0: *norm is
 // given, or folded already: with more partial sums than one launch leaves, every workgroup of every launch would read all
-// of them again, work that grows with the square of the list (bf16 tensors of
-// 100 k elements, folded everywhere / once: 1000 of them 240 / 162 us, 5000 2719 / 858; 300 of 70 k 52 / 51).
+// of them again, work that grows with the square of the list (bf16 tensors of 100 k elements, folded everywhere / once: 1000
+// of them 240 / 162 us, 5000 2719 / 858; 300 of 70 k 52 / 51).
 // A factor of exactly 1 leaves tensors that are scaled in place as they are.
 __global__ __launch_bounds__(NORM_THREADS) void grad_scale_kernel(TensorList list, const double* __restrict__ partial, int partials, int store, double max_norm,
                                                                  double eps, double* norm) {

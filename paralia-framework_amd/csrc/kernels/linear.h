@@ -156,13 +156,13 @@ inline long half_partial_rows(const HalfPlan& p, int type, long M, long N) {
 // Space of the aligned copies of both operands, and their leading dimensions.
 struct Copies { long ld_a, bytes_a, ld_b, bytes_b; long bytes() const { return bytes_a + bytes_b; } };
 
-// fp32 and fp64 operands that are unaligned or ragged are multiplied from copies, because their tile GEMM takes panels straight into LDS only from 16-byte aligned vectors and only in
-// whole tiles and panels: from aligned copies with k filled up by zeros to whole panels and rows to whole tiles of 256, an
-// unaligned product runs at nearly the full rate (3878 x 1869 x 4113 with odd strides, fp32 TN / NN / NT / TT: 970 / 900 /
-// 781 / 900 -> 512 - 552 / 510 / 509 / 508 us, fp64 1092 - 1190 -> 1030), and of aligned operands with ragged edges loses
-// less (3880 x 1872 x 4112: fp32 551 - 598 -> 504, fp64 1076 - 1130 -> 1000 - 1010).  Products that fill less of the device
-// lose less; below the copies' own time there are none.  The space is set aside for whole extents too: their rows may be
-// those of a wider matrix.
+// fp32 and fp64 operands that are unaligned or ragged are multiplied from copies where that pays: their tile GEMM takes
+// panels straight into LDS only from 16-byte aligned vectors and only in whole tiles and panels.  From aligned copies with k
+// filled up by zeros to whole panels and rows to whole tiles of 256, an unaligned product runs at nearly the full rate
+// (3878 x 1869 x 4113 with odd strides, fp32 TN / NN / NT / TT: 970 / 900 / 781 / 900 -> 512 - 552 / 510 / 509 / 508 us, fp64
+// 1092 - 1190 -> 1030), and one of aligned operands with ragged edges loses less (3880 x 1872 x 4112: fp32 551 - 598 -> 504,
+// fp64 1076 - 1130 -> 1000 - 1010).  Products that fill less of the device lose less; below the copies' own time there are
+// none.  The space is set aside for whole extents too: their rows may be those of a wider matrix.
 constexpr long WIDE_ROWS = 256, WIDE_K = 32;
 inline bool wide_aligned(int es, const void* A, long lda, const void* B, long ldb) {
   return aligned_to(A, 16) && aligned_to(B, 16) && lda % (16 / es) == 0 && ldb % (16 / es) == 0;
